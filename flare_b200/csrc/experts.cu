@@ -1,0 +1,652 @@
+// Routed experts around the grouped products: top-k routing with a stable
+// counting sort, SwiGLU with an 8-bit checkpoint, and the combination of the
+// experts' rows.  Everything here is bound by memory or, for a handful of
+// tokens, by the launch; the products are in grouped_gemm.cu.
+//
+// Routing (tokens t = slot * B + b, groups slot * E + e):
+//   chosen experts = the k largest logits, ties to the lowest expert, an expert
+//   at -inf never; w_j = exp(l_j - l_0) / sum_i exp(l_i - l_0) in fp32.
+//   Rows are the (token, choice) pairs sorted by group, within a group by token.
+//   Every count is an integer, so the order does not depend on the schedule.
+// SwiGLU: y = up * gate * sigmoid(gate).  The checkpoint holds up and gate in
+//   e4m3 with one power-of-two scale per 32 columns of a row: dividing by a
+//   power of two is exact, so the only rounding is the one to e4m3.
+// Combination: y_t = sum_j w_tj z[row_of[t, j]], summed in order of j in fp32.
+#include "experts.cuh"
+
+#include <cuda_fp8.h>
+
+#include <algorithm>
+#include <type_traits>
+
+namespace flare {
+namespace {
+
+// ------------------------------------------------------------------ routing
+constexpr int kSub = 256;  // tokens that are ranked together (one bit each)
+
+struct RouteShape {
+  int chunk_tokens;  // tokens of one block, a multiple of kSub
+  int chunks;        // blocks of one slot
+};
+
+// About two blocks per SM: every block of the second pass reads all blocks' counts, so their
+// number is bounded rather than their length.
+RouteShape route_shape(int S, int B) {
+  const int64_t per_slot = std::max<int64_t>(1, 296 / S);
+  int64_t tokens = (B + per_slot - 1) / per_slot;
+  tokens = std::max<int64_t>(kSub, (tokens + kSub - 1) / kSub * kSub);
+  return {static_cast<int>(tokens), static_cast<int>((B + tokens - 1) / tokens)};
+}
+
+// An unsigned key in the order of the logits: NaN above all, -0 equal to +0, -inf at kDeadKey.
+constexpr uint32_t kDeadKey = 0x007FFFFFu;
+__device__ __forceinline__ uint32_t order_key(float v) {
+  if (v != v) return 0xFFFFFFFFu;
+  const uint32_t b = v == 0.f ? 0u : __float_as_uint(v);
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+
+// LANES lanes share a token, each with NV of its experts (expert = v * LANES + lane).
+template <typename T, int LANES, int NV>
+__device__ __forceinline__ void route_pick(const RouteParams& p, int slot, int b, bool live_token, int* hist) {
+  const int sub = threadIdx.x % LANES;
+  const T* row = static_cast<const T*>(p.logits) + slot * p.stride_slot + b * p.stride_token;
+  uint32_t key[NV];
+  float val[NV];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    const int e = v * LANES + sub;
+    const bool in = live_token && e < p.E;
+    val[v] = in ? to_f32(row[e]) : -INFINITY;
+    key[v] = in ? order_key(val[v]) : 0u;
+  }
+  int my_e = -1;  // lane j of the token keeps choice j
+  float my_v = -INFINITY;
+  for (int j = 0; j < p.k; ++j) {
+    uint32_t best = 0;
+    int at = 0;
+    float bv = -INFINITY;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {  // the first of equal keys has the lowest expert
+      if (key[v] > best) best = key[v], at = v * LANES + sub, bv = val[v];
+    }
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) {
+      const uint32_t ob = __shfl_xor_sync(0xffffffffu, best, o);
+      const int oa = __shfl_xor_sync(0xffffffffu, at, o);
+      const float ov = __shfl_xor_sync(0xffffffffu, bv, o);
+      if (ob > best || (ob == best && oa < at)) best = ob, at = oa, bv = ov;
+    }
+    if (sub == j && best > kDeadKey) my_e = at, my_v = bv;
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+      if (v * LANES + sub == at) key[v] = 0u;
+  }
+  const float top = __shfl_sync(0xffffffffu, my_v, 0, LANES);
+  const float mine = my_e >= 0 ? expf(my_v - top) : 0.f;
+  float sum = 0.f;
+  for (int j = 0; j < p.k; ++j) sum += __shfl_sync(0xffffffffu, mine, j, LANES);
+  if (live_token && sub < p.k) {
+    const int64_t i = (static_cast<int64_t>(slot) * p.B + b) * p.k + sub;
+    p.experts[i] = my_e;
+    p.weights[i] = my_e >= 0 ? mine / sum : 0.f;
+    if (my_e >= 0) atomicAdd(hist + my_e, 1);
+  }
+}
+
+// The experts of tokens [b0, b1) of one slot; counts in hist[E] (shared memory, zeroed here).
+template <typename T, int LANES, int NV>
+__device__ __forceinline__ void route_pick_chunk(const RouteParams& p, int slot, int b0, int b1, int* hist) {
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) hist[e] = 0;
+  __syncthreads();
+  const int per = blockDim.x / LANES;
+  for (int b = b0; b < b1; b += per) {  // block-uniform: the picks shuffle across whole warps
+    const int mine = b + threadIdx.x / LANES;
+    route_pick<T, LANES, NV>(p, slot, min(mine, b1 - 1), mine < b1, hist);
+  }
+  __syncthreads();
+}
+
+// Gives every chosen pair of tokens [b0, b1) its row: base[e] (shared) is the next free row of
+// expert e.  The tokens of a sub-block that chose e are bits of mask[e], so a pair's rank is a
+// population count: the order is that of the tokens whatever the threads do.
+__device__ __forceinline__ void route_place_chunk(const RouteParams& p, int slot, int b0, int b1, int* base,
+                                                  uint32_t* mask) {
+  constexpr int W = kSub / 32;
+  for (int s0 = b0; s0 < b1; s0 += kSub) {
+    const int n = min(kSub, b1 - s0) * p.k;
+    const int64_t t0 = static_cast<int64_t>(slot) * p.B + s0;
+    for (int i = threadIdx.x; i < p.E * W; i += blockDim.x) mask[i] = 0u;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+      const int e = p.experts[t0 * p.k + i], b = i / p.k;
+      if (e >= 0) atomicOr(&mask[e * W + (b >> 5)], 1u << (b & 31));
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+      const int e = p.experts[t0 * p.k + i], b = i / p.k;
+      int row = -1;
+      if (e >= 0) {
+        row = base[e] + __popc(mask[e * W + (b >> 5)] & ((1u << (b & 31)) - 1u));
+        for (int w = 0; w < (b >> 5); ++w) row += __popc(mask[e * W + w]);
+        p.rows[row] = static_cast<int>(t0 + b);
+      }
+      p.row_of[t0 * p.k + i] = row;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
+      int c = 0;
+      for (int w = 0; w < W; ++w) c += __popc(mask[e * W + w]);
+      base[e] += c;
+    }
+    __syncthreads();
+  }
+}
+
+// Exclusive prefix of tot[E] in place by one warp; returns the total to every lane.
+__device__ __forceinline__ int warp_exclusive(int* tot, int E) {
+  const int lane = lane_id();
+  int carry = 0;
+  for (int e0 = 0; e0 < E; e0 += 32) {
+    const int c = e0 + lane < E ? tot[e0 + lane] : 0;
+    int inc = c;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += up;
+    }
+    if (e0 + lane < E) tot[e0 + lane] = carry + inc - c;
+    carry += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  return carry;
+}
+
+// Pass 1: experts and weights of every token, and each block's counts: work[block][E + 1] (the
+// last entry is their sum).
+template <typename T, int LANES, int NV>
+__global__ void __launch_bounds__(256) route_pick_kernel(RouteParams p, RouteShape sh) {
+  __shared__ int hist[kRouteMaxExperts];
+  __shared__ int sum;
+  const int slot = blockIdx.x / sh.chunks, c = blockIdx.x % sh.chunks;
+  if (threadIdx.x == 0) sum = 0;
+  route_pick_chunk<T, LANES, NV>(p, slot, c * sh.chunk_tokens, min(p.B, (c + 1) * sh.chunk_tokens), hist);
+  int* out = p.work + static_cast<int64_t>(blockIdx.x) * (p.E + 1);
+  int mine = 0;
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) out[e] = hist[e], mine += hist[e];
+  if (mine) atomicAdd(&sum, mine);
+  __syncthreads();
+  if (threadIdx.x == 0) out[p.E] = sum;
+}
+
+// Pass 2: a block's first row of each expert = rows of the slots before + of the experts before
+// + of the blocks before; then its pairs' rows.
+__global__ void __launch_bounds__(256) route_place_kernel(RouteParams p, RouteShape sh) {
+  __shared__ int tot[kRouteMaxExperts], pre[kRouteMaxExperts];
+  __shared__ uint32_t mask[kRouteMaxExperts * (kSub / 32)];
+  __shared__ int before, total;
+  const int slot = blockIdx.x / sh.chunks, c = blockIdx.x % sh.chunks;
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) tot[e] = pre[e] = 0;
+  if (threadIdx.x == 0) before = total = 0;
+  __syncthreads();
+  int bsum = 0, tsum = 0;
+  for (int i = threadIdx.x; i < static_cast<int>(gridDim.x); i += blockDim.x) {
+    const int v = p.work[static_cast<int64_t>(i) * (p.E + 1) + p.E];
+    tsum += v;
+    if (i / sh.chunks < slot) bsum += v;
+  }
+  if (bsum) atomicAdd(&before, bsum);
+  if (tsum) atomicAdd(&total, tsum);
+  const int* mine = p.work + static_cast<int64_t>(slot) * sh.chunks * (p.E + 1);
+  // thread = expert where there are many, several blocks at a time where there are few
+  const int parts = max(1, static_cast<int>(blockDim.x) / p.E);
+  for (int i = threadIdx.x; i < parts * p.E; i += blockDim.x) {
+    const int e = i % p.E;
+    int a = 0, b = 0;
+    for (int q = i / p.E; q < sh.chunks; q += parts) {
+      const int v = mine[static_cast<int64_t>(q) * (p.E + 1) + e];
+      a += v;
+      if (q < c) b += v;
+    }
+    if (a) atomicAdd(&tot[e], a);
+    if (b) atomicAdd(&pre[e], b);
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) warp_exclusive(tot, p.E);
+  __syncthreads();
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
+    const int first = before + tot[e];
+    if (c == 0) p.offsets[slot * p.E + e] = first;
+    pre[e] += first;
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) p.offsets[p.S * p.E] = total;
+  const int64_t R = static_cast<int64_t>(p.S) * p.B * p.k;
+  for (int64_t i = total + static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < R;
+       i += static_cast<int64_t>(gridDim.x) * blockDim.x)
+    p.rows[i] = -1;
+  __syncthreads();
+  route_place_chunk(p, slot, c * sh.chunk_tokens, min(p.B, (c + 1) * sh.chunk_tokens), pre, mask);
+}
+
+// Both passes in one block: one slot of at most kRouteOneBlock tokens.
+constexpr int kRouteOneBlock = 512;
+template <typename T, int LANES, int NV>
+__global__ void __launch_bounds__(512) route_one_kernel(RouteParams p) {
+  __shared__ int hist[kRouteMaxExperts];
+  __shared__ uint32_t mask[kRouteMaxExperts * (kSub / 32)];
+  __shared__ int total;
+  route_pick_chunk<T, LANES, NV>(p, 0, 0, p.B, hist);
+  if (threadIdx.x < 32) {
+    const int t = warp_exclusive(hist, p.E);
+    if (threadIdx.x == 0) total = t;
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) p.offsets[e] = hist[e];
+  if (threadIdx.x == 0) p.offsets[p.E] = total;
+  for (int i = total + threadIdx.x; i < p.B * p.k; i += blockDim.x) p.rows[i] = -1;
+  __syncthreads();
+  route_place_chunk(p, 0, 0, p.B, hist, mask);
+}
+
+template <typename T, int LANES, int NV>
+void route_launch(const RouteParams& p, cudaStream_t s) {
+  if (p.S == 1 && p.B <= kRouteOneBlock) {
+    // enough threads for every token at once, 512 at most
+    const int threads = std::min(512, std::max(64, ceil_div(static_cast<int64_t>(p.B) * LANES, 32) * 32));
+    route_one_kernel<T, LANES, NV><<<1, threads, 0, s>>>(p);
+    FLARE_CUDA_CHECK(cudaGetLastError());
+    count_launch();
+    return;
+  }
+  const RouteShape sh = route_shape(p.S, p.B);
+  route_pick_kernel<T, LANES, NV><<<p.S * sh.chunks, 256, 0, s>>>(p, sh);
+  FLARE_CUDA_CHECK(cudaGetLastError());
+  route_place_kernel<<<p.S * sh.chunks, 256, 0, s>>>(p, sh);
+  FLARE_CUDA_CHECK(cudaGetLastError());
+  count_launch(2);
+}
+
+template <typename T>
+void route_typed(const RouteParams& p, cudaStream_t s) {
+  if (p.E <= 8) route_launch<T, 8, 1>(p, s);
+  else if (p.E <= 16) route_launch<T, 16, 1>(p, s);
+  else if (p.E <= 32) route_launch<T, 32, 1>(p, s);
+  else if (p.E <= 64) route_launch<T, 32, 2>(p, s);
+  else if (p.E <= 128) route_launch<T, 32, 4>(p, s);
+  else if (p.E <= 256) route_launch<T, 32, 8>(p, s);
+  else route_launch<T, 32, 16>(p, s);
+}
+
+// d logits[t, e] = w_j (dw_j - sum_i w_i dw_i) where choice j of t is e, else 0.
+template <typename T>
+__global__ void __launch_bounds__(256) route_bwd_kernel(RouteBwdParams p, int lanes) {
+  const int sub = threadIdx.x % lanes;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * (blockDim.x / lanes);
+  for (int64_t t = static_cast<int64_t>(blockIdx.x) * (blockDim.x / lanes) + threadIdx.x / lanes; t < p.T; t += step) {
+    const int* ex = p.experts + t * p.k;
+    const float* w = p.weights + t * p.k;
+    const float* dw = p.dweights + t * p.k;
+    float dot = 0.f;
+    for (int j = 0; j < p.k; ++j) dot += ex[j] >= 0 ? w[j] * dw[j] : 0.f;
+    T* out = static_cast<T*>(p.dlogits) + t * p.E;
+    for (int e = sub; e < p.E; e += lanes) {
+      float g = 0.f;
+      for (int j = 0; j < p.k; ++j)
+        if (ex[j] == e) g = w[j] * (dw[j] - dot);
+      out[e] = from_f32<T>(g);
+    }
+  }
+}
+
+// ----------------------------------------------------------------- vectors
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Vec {
+  T v[N];
+};
+
+template <typename T, int N>
+__device__ __forceinline__ void load_f(const T* p, float (&f)[N]) {
+  const Vec<T, N> u = *reinterpret_cast<const Vec<T, N>*>(p);
+#pragma unroll
+  for (int i = 0; i < N; ++i) f[i] = to_f32(u.v[i]);
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_f(T* p, const float (&f)[N]) {
+  Vec<T, N> u;
+#pragma unroll
+  for (int i = 0; i < N; ++i) u.v[i] = from_f32<T>(f[i]);
+  *reinterpret_cast<Vec<T, N>*>(p) = u;
+}
+
+// ------------------------------------------------------------------ SwiGLU
+constexpr int kGroupCols = 32;
+
+// sigmoid: outputs of 16 bits lose nothing to the fast exponential (2 ulp of fp32 and more for
+// large arguments) and division; fp32 outputs take the accurate ones.
+template <bool kFast>
+__device__ __forceinline__ float sigmoid_f(float g) {
+  if constexpr (kFast) return __fdividef(1.f, 1.f + __expf(-g));
+  return 1.f / (1.f + expf(-g));
+}
+
+// The scale exponent of a group whose largest finite magnitude is `top`: the largest value lands
+// in (224, 448], 448 being e4m3's largest.  -126 keeps the scale's inverse finite.
+__device__ __forceinline__ int scale_exponent(float top) {
+  const uint32_t b = __float_as_uint(top);
+  const int x = static_cast<int>(b >> 23) - 127;  // floor(log2(top)), or -127 below 2^-126
+  return max((b & 0x007FFFFFu) <= 0x00600000u ? x - 8 : x - 7, -126);
+}
+__device__ __forceinline__ float exp2_int(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+
+__device__ __forceinline__ float finite_abs(float v) {
+  const float a = fabsf(v);
+  return a < INFINITY ? a : 0.f;  // NaN and infinities say nothing about the others
+}
+
+// e4m3 of v * inv; infinities become NaN (e4m3 has no infinity), NaN stays.
+template <int N>
+__device__ __forceinline__ void pack_e4m3(const float (&v)[N], float inv, uint8_t* out) {
+  Vec<uint8_t, N> u;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const bool inf = fabsf(v[i]) == INFINITY;
+    u.v[i] = inf ? 0x7F : static_cast<uint8_t>(__nv_cvt_float_to_fp8(v[i] * inv, __NV_SATFINITE, __NV_E4M3));
+  }
+  *reinterpret_cast<Vec<uint8_t, N>*>(out) = u;
+}
+template <int N>
+__device__ __forceinline__ void unpack_e4m3(const uint8_t* in, float scale, float (&v)[N]) {
+  const Vec<uint8_t, N> u = *reinterpret_cast<const Vec<uint8_t, N>*>(in);
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = __half2float(__half(__nv_cvt_fp8_to_halfraw(u.v[i], __NV_E4M3))) * scale;
+}
+
+// A thread owns N consecutive columns of up and the same of gate; kGroupCols / N lanes share a
+// scale.  A row's columns are padded to whole scale groups (`cols` chunks of N), short rows share
+// a block.  One pass: x is read once, y and the checkpoint are written once.
+struct RowTiling {
+  int cols;  // chunks per row, padded to whole scale groups
+  int rows;  // rows of one block step (1 where a row fills the block)
+};
+
+template <typename T, int N, bool kKeep>
+__global__ void __launch_bounds__(256) swiglu_fwd_kernel(SwigluParams p, RowTiling t) {
+  constexpr int GL = kGroupCols / N;
+  const int r0 = t.rows > 1 ? threadIdx.x / t.cols : 0;
+  const int c0 = t.rows > 1 ? threadIdx.x % t.cols : threadIdx.x;
+  const int64_t groups = (p.h + kGroupCols - 1) / kGroupCols;
+  for (int64_t rb = static_cast<int64_t>(blockIdx.x) * t.rows; rb < p.R; rb += static_cast<int64_t>(gridDim.x) * t.rows) {
+    const int64_t r = rb + r0;
+    const bool row_in = r0 < t.rows && r < p.R;
+    for (int cb = 0; cb < t.cols; cb += 256) {  // block-uniform: the scales are shared by shuffles
+      const int c = c0 + cb;
+      const int64_t col = static_cast<int64_t>(c) * N;
+      const bool in = row_in && col < p.h;
+      float up[N], gate[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) up[i] = gate[i] = 0.f;
+      if (in) {
+        const T* x = static_cast<const T*>(p.x) + r * p.ldx + col;
+        load_f<T, N>(x, up);
+        load_f<T, N>(x + p.h, gate);
+        float y[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) y[i] = up[i] * (gate[i] * sigmoid_f<sizeof(T) == 2>(gate[i]));
+        store_f<T, N>(static_cast<T*>(p.y) + r * p.h + col, y);
+      }
+      if constexpr (kKeep) {
+        float tu = 0.f, tg = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) tu = fmaxf(tu, finite_abs(up[i])), tg = fmaxf(tg, finite_abs(gate[i]));
+#pragma unroll
+        for (int o = GL / 2; o > 0; o >>= 1) {
+          tu = fmaxf(tu, __shfl_xor_sync(0xffffffffu, tu, o));
+          tg = fmaxf(tg, __shfl_xor_sync(0xffffffffu, tg, o));
+        }
+        if (in) {
+          const int eu = scale_exponent(tu), eg = scale_exponent(tg);
+          uint8_t* q = p.q + r * 2 * p.h + col;
+          pack_e4m3<N>(up, exp2_int(-eu), q);
+          pack_e4m3<N>(gate, exp2_int(-eg), q + p.h);
+          if (c % GL == 0) {
+            uint8_t* sc = p.scale + r * 2 * groups + c / GL;
+            sc[0] = static_cast<uint8_t>(eu + 127);
+            sc[groups] = static_cast<uint8_t>(eg + 127);
+          }
+        }
+      }
+    }
+  }
+}
+
+// d up = dy * gate * s, d gate = dy * up * s * (1 + gate * (1 - s)), s = sigmoid(gate), from x
+// itself or from the values that the checkpoint stands for.  The factors of s come first: a large
+// negative gate makes them 0 before the others can overflow.
+template <typename T, int N, bool kKeep>
+__global__ void __launch_bounds__(256) swiglu_bwd_kernel(SwigluParams p, RowTiling t) {
+  constexpr int GL = kGroupCols / N;
+  const int r0 = t.rows > 1 ? threadIdx.x / t.cols : 0;
+  const int c0 = t.rows > 1 ? threadIdx.x % t.cols : threadIdx.x;
+  const int64_t groups = (p.h + kGroupCols - 1) / kGroupCols;
+  for (int64_t rb = static_cast<int64_t>(blockIdx.x) * t.rows; rb < p.R; rb += static_cast<int64_t>(gridDim.x) * t.rows) {
+    const int64_t r = rb + r0;
+    if (r0 >= t.rows || r >= p.R) continue;
+    for (int c = c0; c < t.cols; c += 256) {
+      const int64_t col = static_cast<int64_t>(c) * N;
+      if (col >= p.h) continue;
+      float up[N], gate[N], dy[N], du[N], dg[N];
+      if constexpr (kKeep) {
+        const uint8_t* q = p.q + r * 2 * p.h + col;
+        const uint8_t* sc = p.scale + r * 2 * groups + c / GL;
+        unpack_e4m3<N>(q, exp2_int(static_cast<int>(sc[0]) - 127), up);
+        unpack_e4m3<N>(q + p.h, exp2_int(static_cast<int>(sc[groups]) - 127), gate);
+      } else {
+        const T* x = static_cast<const T*>(p.x) + r * p.ldx + col;
+        load_f<T, N>(x, up);
+        load_f<T, N>(x + p.h, gate);
+      }
+      load_f<T, N>(static_cast<const T*>(p.dy) + r * p.lddy + col, dy);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float s = sigmoid_f<sizeof(T) == 2>(gate[i]);
+        du[i] = dy[i] * (gate[i] * s);
+        dg[i] = dy[i] * (up[i] * (s * (1.f + gate[i] * (1.f - s))));
+      }
+      T* dx = static_cast<T*>(p.dx) + r * 2 * p.h + col;
+      store_f<T, N>(dx, du);
+      store_f<T, N>(dx + p.h, dg);
+    }
+  }
+}
+
+template <typename T, int N>
+void swiglu_launch(const SwigluParams& p, bool backward, cudaStream_t s) {
+  constexpr int GL = kGroupCols / N;
+  RowTiling t;
+  t.cols = static_cast<int>((p.h + kGroupCols - 1) / kGroupCols) * GL;
+  t.rows = t.cols <= 128 ? 256 / t.cols : 1;
+  const int grid = static_cast<int>(std::min<int64_t>((p.R + t.rows - 1) / t.rows, 148 * 16));
+  if (!backward) {
+    if (p.q != nullptr) swiglu_fwd_kernel<T, N, true><<<grid, 256, 0, s>>>(p, t);
+    else swiglu_fwd_kernel<T, N, false><<<grid, 256, 0, s>>>(p, t);
+  } else {
+    if (p.q != nullptr) swiglu_bwd_kernel<T, N, true><<<grid, 256, 0, s>>>(p, t);
+    else swiglu_bwd_kernel<T, N, false><<<grid, 256, 0, s>>>(p, t);
+  }
+  FLARE_CUDA_CHECK(cudaGetLastError());
+  count_launch();
+}
+
+bool vec_ok(const void* p, int64_t ld, int dtype) {
+  const int es = dtype == kF32 ? 4 : 2;
+  return p == nullptr || ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * es) % 16 == 0);
+}
+
+void swiglu_dispatch(const SwigluParams& p, bool backward, cudaStream_t s) {
+  if (p.R == 0 || p.h == 0) return;
+  // 16-byte vectors where rows and halves start on 16 bytes, single elements elsewhere
+  const int64_t per = p.dtype == kF32 ? 4 : 8;
+  const bool vec = p.h % per == 0 && vec_ok(p.x, p.ldx, p.dtype) && (!backward || vec_ok(p.dy, p.lddy, p.dtype));
+  switch (p.dtype) {
+    case kF32: vec ? swiglu_launch<float, 4>(p, backward, s) : swiglu_launch<float, 1>(p, backward, s); break;
+    case kBF16: vec ? swiglu_launch<__nv_bfloat16, 8>(p, backward, s) : swiglu_launch<__nv_bfloat16, 1>(p, backward, s); break;
+    default: vec ? swiglu_launch<__half, 8>(p, backward, s) : swiglu_launch<__half, 1>(p, backward, s); break;
+  }
+}
+
+// ------------------------------------------------------------- combination
+// A thread owns N columns of one token and reads its k rows one after another (four in flight).
+template <typename T, int N, typename O>
+__global__ void __launch_bounds__(256) combine_fwd_kernel(CombineParams p, RowTiling t) {
+  const int r0 = t.rows > 1 ? threadIdx.x / t.cols : 0;
+  const int c0 = t.rows > 1 ? threadIdx.x % t.cols : threadIdx.x;
+  if (r0 >= t.rows) return;
+  for (int64_t tb = static_cast<int64_t>(blockIdx.x) * t.rows; tb < p.T; tb += static_cast<int64_t>(gridDim.x) * t.rows) {
+    const int64_t tok = tb + r0;
+    if (tok >= p.T) continue;
+    const int* rows = p.row_of + tok * p.k;
+    for (int c = c0; c < t.cols; c += 256) {
+      float acc[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) acc[i] = 0.f;
+      for (int j0 = 0; j0 < p.k; j0 += 4) {
+        float f[4][N];
+        float w[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int row = j0 + q < p.k ? rows[j0 + q] : -1;
+          w[q] = 0.f;
+          if (row >= 0 && row < p.R) {
+            load_f<T, N>(static_cast<const T*>(p.z) + row * p.ldz + static_cast<int64_t>(c) * N, f[q]);
+            w[q] = p.weights != nullptr ? p.weights[tok * p.k + j0 + q] : 1.f;
+          } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) f[q][i] = 0.f;
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int i = 0; i < N; ++i) acc[i] = fmaf(w[q], f[q][i], acc[i]);
+      }
+      store_f<O, N>(static_cast<O*>(p.y) + tok * p.N + static_cast<int64_t>(c) * N, acc);
+    }
+  }
+}
+
+// A warp per (token, choice): dz[row] = w * dy[t], dw = <z[row], dy[t]>; a token's choices are
+// neighbours, so its dy comes from the caches.  Rows behind the last group get zeros.  Without
+// weights dz[row] = dy[t] and z is not read.
+template <typename T, int N>
+__global__ void __launch_bounds__(256) combine_bwd_kernel(CombineParams p) {
+  const int lane = lane_id();
+  const int64_t warps = static_cast<int64_t>(gridDim.x) * 8, pairs = p.T * p.k;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + warp_id(); i < pairs; i += warps) {
+    const int row = p.row_of[i];
+    if (row < 0 || row >= p.R) {
+      if (lane == 0 && p.dw != nullptr) p.dw[i] = 0.f;
+      continue;
+    }
+    const int64_t tok = i / p.k;
+    const float w = p.weights != nullptr ? p.weights[i] : 1.f;
+    const T* dy = static_cast<const T*>(p.dy) + tok * p.lddy;
+    const T* z = static_cast<const T*>(p.z) + row * p.ldz;
+    T* dz = static_cast<T*>(p.dz) + static_cast<int64_t>(row) * p.N;
+    float dot = 0.f;
+#pragma unroll 2
+    for (int c = lane * N; c < p.N; c += 32 * N) {
+      float a[N], o[N];
+      load_f<T, N>(dy + c, a);
+#pragma unroll
+      for (int q = 0; q < N; ++q) o[q] = w * a[q];
+      store_f<T, N>(dz + c, o);
+      if (p.dw != nullptr) {
+        float b[N];
+        load_f<T, N>(z + c, b);
+#pragma unroll
+        for (int q = 0; q < N; ++q) dot = fmaf(a[q], b[q], dot);
+      }
+    }
+    if (p.dw == nullptr) continue;
+    dot = warp_sum(dot);
+    if (lane == 0) p.dw[i] = dot;
+  }
+  const int64_t total = max(0, *p.total);
+  for (int64_t r = total + static_cast<int64_t>(blockIdx.x) * 8 + warp_id(); r < p.R; r += warps) {
+    float zero[N];
+#pragma unroll
+    for (int q = 0; q < N; ++q) zero[q] = 0.f;
+    for (int c = lane * N; c < p.N; c += 32 * N) store_f<T, N>(static_cast<T*>(p.dz) + r * p.N + c, zero);
+  }
+}
+
+template <typename T, int N>
+void combine_launch(const CombineParams& p, bool backward, cudaStream_t s) {
+  if (!backward) {
+    RowTiling t;
+    t.cols = p.N / N;
+    t.rows = t.cols <= 128 ? 256 / t.cols : 1;
+    const int grid = static_cast<int>(std::min<int64_t>((p.T + t.rows - 1) / t.rows, 148 * 16));
+    if constexpr (sizeof(T) == 4) {
+      if (p.out_dtype == kBF16) combine_fwd_kernel<T, N, __nv_bfloat16><<<grid, 256, 0, s>>>(p, t);
+      else if (p.out_dtype == kF16) combine_fwd_kernel<T, N, __half><<<grid, 256, 0, s>>>(p, t);
+      else combine_fwd_kernel<T, N, T><<<grid, 256, 0, s>>>(p, t);
+    } else {
+      combine_fwd_kernel<T, N, T><<<grid, 256, 0, s>>>(p, t);
+    }
+  } else {
+    const int grid = static_cast<int>(std::min<int64_t>((std::max(p.T * p.k, p.R) + 7) / 8, 148 * 16));
+    combine_bwd_kernel<T, N><<<grid, 256, 0, s>>>(p);
+  }
+  FLARE_CUDA_CHECK(cudaGetLastError());
+  count_launch();
+}
+
+void combine_dispatch(const CombineParams& p, bool backward, cudaStream_t s) {
+  if (p.N == 0 || (p.T == 0 && !(backward && p.R > 0))) return;
+  const int per = p.dtype == kF32 ? 4 : 8;
+  const bool vec = p.N % per == 0 && vec_ok(p.z, p.ldz, p.dtype) && (!backward || vec_ok(p.dy, p.lddy, p.dtype));
+  switch (p.dtype) {
+    case kF32: vec ? combine_launch<float, 4>(p, backward, s) : combine_launch<float, 1>(p, backward, s); break;
+    case kBF16: vec ? combine_launch<__nv_bfloat16, 8>(p, backward, s) : combine_launch<__nv_bfloat16, 1>(p, backward, s); break;
+    default: vec ? combine_launch<__half, 8>(p, backward, s) : combine_launch<__half, 1>(p, backward, s); break;
+  }
+}
+
+}  // namespace
+
+int64_t route_work_ints(int S, int B, int E) {
+  if (S == 1 && B <= kRouteOneBlock) return 0;
+  return static_cast<int64_t>(S) * route_shape(S, B).chunks * (E + 1);
+}
+
+void route_topk(const RouteParams& p, cudaStream_t s) {
+  FLARE_CHECK(p.S > 0 && p.B > 0, "route_topk: no tokens");
+  FLARE_CHECK(p.E > 0 && p.E <= kRouteMaxExperts, "route_topk: 1 to 512 experts");
+  FLARE_CHECK(p.k > 0 && p.k <= p.E && p.k <= kRouteMaxTopK, "route_topk: top_k is at most the experts, and 32");
+  switch (p.dtype) {
+    case kF32: route_typed<float>(p, s); break;
+    case kBF16: route_typed<__nv_bfloat16>(p, s); break;
+    default: route_typed<__half>(p, s); break;
+  }
+}
+
+void route_topk_backward(const RouteBwdParams& p, cudaStream_t s) {
+  if (p.T == 0) return;
+  const int lanes = p.E <= 8 ? 8 : p.E <= 16 ? 16 : 32;
+  const int grid = static_cast<int>(std::min<int64_t>((p.T + 256 / lanes - 1) / (256 / lanes), 148 * 16));
+  switch (p.dtype) {
+    case kF32: route_bwd_kernel<float><<<grid, 256, 0, s>>>(p, lanes); break;
+    case kBF16: route_bwd_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(p, lanes); break;
+    default: route_bwd_kernel<__half><<<grid, 256, 0, s>>>(p, lanes); break;
+  }
+  FLARE_CUDA_CHECK(cudaGetLastError());
+  count_launch();
+}
+
+void swiglu_forward(const SwigluParams& p, cudaStream_t s) { swiglu_dispatch(p, false, s); }
+void swiglu_backward(const SwigluParams& p, cudaStream_t s) { swiglu_dispatch(p, true, s); }
+void combine_forward(const CombineParams& p, cudaStream_t s) { combine_dispatch(p, false, s); }
+void combine_backward(const CombineParams& p, cudaStream_t s) { combine_dispatch(p, true, s); }
+
+}  // namespace flare

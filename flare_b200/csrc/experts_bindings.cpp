@@ -1,0 +1,512 @@
+// The routed-expert operators as autograd functions, and their Python bindings.
+// They take tensors and allocate their outputs and scratch from the caching
+// allocator on the current stream: scratch that belongs to one call cannot be
+// shared by two captured graphs.  For a few tokens the call itself is what
+// counts, so the graph nodes are C++ (a Python node costs some 40 us a step).  Arguments are checked by
+// flare_b200/ops/experts.py; what is checked here again is what a wrong pointer
+// or size would cost.
+#include <torch/extension.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+
+#include "experts.cuh"
+
+namespace py = pybind11;
+using at::Tensor;
+using c10::optional;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+namespace {
+
+int code_of(at::ScalarType t) {
+  if (t == at::kFloat) return flare::kF32;
+  if (t == at::kBFloat16) return flare::kBF16;
+  TORCH_CHECK(t == at::kHalf, "expected float32, bfloat16 or float16, got ", t);
+  return flare::kF16;
+}
+
+cudaStream_t stream() { return at::cuda::getCurrentCUDAStream().stream(); }
+
+Tensor empty(at::IntArrayRef sizes, const Tensor& like, at::ScalarType t) {
+  return at::empty(sizes, like.options().dtype(t));
+}
+
+// 2-D rows of unit inner stride
+void check_rows(const Tensor& t, const char* what) {
+  TORCH_CHECK(t.is_cuda() && t.dim() == 2 && (t.stride(1) == 1 || t.size(1) <= 1), what, ": rows of unit inner stride on a CUDA device");
+}
+int64_t pitch(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+const int* ints(const Tensor& t, const Tensor& like, int64_t n, const char* what) {
+  TORCH_CHECK(t.scalar_type() == at::kInt && t.is_contiguous() && t.device() == like.device() && t.numel() == n, what,
+              ": int32, contiguous, on the same device, with ", n, " values");
+  return t.data_ptr<int>();
+}
+
+// logits [S, B, E] of unit inner stride
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> route_topk(const Tensor& logits, int64_t k) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 3, "route_topk: logits [slots, tokens, experts] on a CUDA device");
+  const c10::cuda::CUDAGuard guard(logits.device());
+  const int64_t S = logits.size(0), B = logits.size(1), E = logits.size(2);
+  TORCH_CHECK(E >= 1 && E <= flare::kRouteMaxExperts, "route_topk: 1 to 512 experts, got ", E);
+  TORCH_CHECK(k >= 1 && k <= E && k <= flare::kRouteMaxTopK, "route_topk: top_k from 1 to the number of experts and 32, got ", k);
+  TORCH_CHECK(S * E < (1ll << 31) - 1 && S * B * k < (1ll << 31) - 512, "route_topk: too many rows");
+  TORCH_CHECK(E == 1 || logits.stride(2) == 1, "route_topk: logits need unit inner stride");
+  Tensor experts = empty({S, B, k}, logits, at::kInt), weights = empty({S, B, k}, logits, at::kFloat);
+  Tensor offsets = empty({S * E + 1}, logits, at::kInt), rows = empty({S * B * k}, logits, at::kInt);
+  Tensor row_of = empty({S, B, k}, logits, at::kInt);
+  if (S * B == 0) {
+    offsets.zero_();
+    return {experts, weights, offsets, rows, row_of};
+  }
+  flare::RouteParams p{};
+  p.logits = logits.data_ptr();
+  p.stride_slot = logits.stride(0);
+  p.stride_token = logits.stride(1);
+  p.dtype = code_of(logits.scalar_type());
+  p.S = static_cast<int>(S);
+  p.B = static_cast<int>(B);
+  p.E = static_cast<int>(E);
+  p.k = static_cast<int>(k);
+  p.experts = experts.data_ptr<int>();
+  p.weights = weights.data_ptr<float>();
+  p.offsets = offsets.data_ptr<int>();
+  p.rows = rows.data_ptr<int>();
+  p.row_of = row_of.data_ptr<int>();
+  const int64_t ints_needed = flare::route_work_ints(p.S, p.B, p.E);
+  Tensor work;
+  if (ints_needed > 0) {
+    work = empty({ints_needed}, logits, at::kInt);
+    p.work = work.data_ptr<int>();
+  }
+  flare::route_topk(p, stream());
+  return {experts, weights, offsets, rows, row_of};
+}
+
+Tensor route_topk_backward(const Tensor& experts, const Tensor& weights, const Tensor& dweights, int64_t E, at::ScalarType dtype) {
+  const c10::cuda::CUDAGuard guard(experts.device());
+  const int64_t k = experts.size(2), T = experts.size(0) * experts.size(1);
+  TORCH_CHECK(weights.is_contiguous() && dweights.is_contiguous() && dweights.scalar_type() == at::kFloat && dweights.numel() == T * k,
+              "route_topk: gradient of the weights");
+  Tensor d = empty({experts.size(0), experts.size(1), E}, experts, dtype);
+  flare::RouteBwdParams p{};
+  p.experts = ints(experts, experts, T * k, "experts");
+  p.weights = weights.data_ptr<float>();
+  p.dweights = dweights.data_ptr<float>();
+  p.T = T;
+  p.E = static_cast<int>(E);
+  p.k = static_cast<int>(k);
+  p.dlogits = d.data_ptr();
+  p.dtype = code_of(dtype);
+  flare::route_topk_backward(p, stream());
+  return d;
+}
+
+flare::SwigluParams swiglu_params(const Tensor& x) {
+  check_rows(x, "swiglu");
+  TORCH_CHECK(x.size(1) % 2 == 0, "swiglu: an even number of columns [up | gate], got ", x.size(1));
+  flare::SwigluParams p{};
+  p.x = x.data_ptr();
+  p.ldx = pitch(x);
+  p.R = x.size(0);
+  p.h = x.size(1) / 2;
+  p.dtype = code_of(x.scalar_type());
+  return p;
+}
+
+// (y, q, scale); q and scale are empty without a checkpoint
+std::tuple<Tensor, Tensor, Tensor> swiglu_forward(const Tensor& x, bool keep) {
+  flare::SwigluParams p = swiglu_params(x);
+  const c10::cuda::CUDAGuard guard(x.device());
+  Tensor y = empty({p.R, p.h}, x, x.scalar_type()), q, scale;
+  p.y = y.data_ptr();
+  if (keep) {
+    q = empty({p.R, 2 * p.h}, x, at::kByte);
+    scale = empty({p.R, 2 * ((p.h + 31) / 32)}, x, at::kByte);
+    p.q = q.data_ptr<uint8_t>();
+    p.scale = scale.data_ptr<uint8_t>();
+  }
+  flare::swiglu_forward(p, stream());
+  return {y, q, scale};
+}
+
+// from x, or from the checkpoint (q, scale) that the forward pass kept
+Tensor swiglu_backward(const optional<Tensor>& x, const optional<Tensor>& q, const optional<Tensor>& scale, const Tensor& dy) {
+  check_rows(dy, "swiglu gradient");
+  const c10::cuda::CUDAGuard guard(dy.device());
+  flare::SwigluParams p{};
+  if (x.has_value()) {
+    p = swiglu_params(*x);
+    TORCH_CHECK(x->scalar_type() == dy.scalar_type(), "swiglu: type of the gradient");
+  } else {
+    p.R = dy.size(0);
+    p.h = dy.size(1);
+    p.dtype = code_of(dy.scalar_type());
+    TORCH_CHECK(q.has_value() && scale.has_value() && q->is_contiguous() && scale->is_contiguous() && q->numel() == 2 * p.R * p.h &&
+                    scale->numel() == p.R * 2 * ((p.h + 31) / 32),
+                "swiglu: checkpoint of another size");
+    p.q = q->data_ptr<uint8_t>();
+    p.scale = scale->data_ptr<uint8_t>();
+  }
+  TORCH_CHECK(dy.size(0) == p.R && dy.size(1) == p.h, "swiglu: gradient of another size");
+  Tensor dx = empty({p.R, 2 * p.h}, dy, dy.scalar_type());
+  p.dy = dy.data_ptr();
+  p.lddy = pitch(dy);
+  p.dx = dx.data_ptr();
+  flare::swiglu_backward(p, stream());
+  return dx;
+}
+
+// y [T, N] from z [R, N]; row_of [T, k]; weights fp32 [T, k] or none (plain sum)
+Tensor combine_forward(const Tensor& z, const Tensor& row_of, const optional<Tensor>& weights, int64_t T, int64_t k, at::ScalarType out) {
+  check_rows(z, "combine_rows");
+  const c10::cuda::CUDAGuard guard(z.device());
+  flare::CombineParams p{};
+  p.z = z.data_ptr();
+  p.ldz = pitch(z);
+  p.row_of = ints(row_of, z, T * k, "row_of");
+  if (weights.has_value()) {
+    TORCH_CHECK(weights->scalar_type() == at::kFloat && weights->is_contiguous() && weights->numel() == T * k && weights->device() == z.device(),
+                "combine_rows: weights are float32, contiguous, one for each choice");
+    p.weights = weights->data_ptr<float>();
+  }
+  p.T = T;
+  p.R = z.size(0);
+  TORCH_CHECK(z.size(1) < (1ll << 31) - 4096, "combine_rows: too wide");
+  p.N = static_cast<int>(z.size(1));
+  p.k = static_cast<int>(k);
+  p.dtype = code_of(z.scalar_type());
+  TORCH_CHECK(out == z.scalar_type() || z.scalar_type() == at::kFloat, "combine_rows: type of the result");
+  p.out_dtype = code_of(out);
+  Tensor y = empty({T, z.size(1)}, z, out);
+  p.y = y.data_ptr();
+  flare::combine_forward(p, stream());
+  return y;
+}
+
+// (dz, dw); without weights every row's gradient is its token's, and dw is none
+std::tuple<Tensor, optional<Tensor>> combine_backward(const optional<Tensor>& z, const Tensor& row_of, const optional<Tensor>& weights,
+                                                      const Tensor& offsets, const Tensor& dy, int64_t R, int64_t T, int64_t k) {
+  check_rows(dy, "combine_rows gradient");
+  const c10::cuda::CUDAGuard guard(dy.device());
+  const int64_t N = dy.size(1);
+  TORCH_CHECK(dy.size(0) == T && N < (1ll << 31) - 4096, "combine_rows: gradient of another size");
+  flare::CombineParams p{};
+  p.row_of = ints(row_of, dy, T * k, "row_of");
+  p.T = T;
+  p.R = R;
+  p.N = static_cast<int>(N);
+  p.k = static_cast<int>(k);
+  p.dtype = code_of(dy.scalar_type());
+  p.dy = dy.data_ptr();
+  p.lddy = pitch(dy);
+  Tensor dz = empty({R, N}, dy, dy.scalar_type());
+  p.dz = dz.data_ptr();
+  p.total = ints(offsets, dy, offsets.numel(), "offsets") + offsets.numel() - 1;
+  optional<Tensor> dw;
+  if (weights.has_value()) {
+    TORCH_CHECK(z.has_value(), "combine_rows: the weights' gradient needs the rows");
+    check_rows(*z, "combine_rows");
+    TORCH_CHECK(z->size(0) == R && z->size(1) == N && z->scalar_type() == dy.scalar_type() && weights->is_contiguous() &&
+                    weights->scalar_type() == at::kFloat && weights->numel() == T * k,
+                "combine_rows: gradient of another size or type");
+    p.z = z->data_ptr();
+    p.ldz = pitch(*z);
+    p.weights = weights->data_ptr<float>();
+    dw = empty({T * k}, dy, at::kFloat);
+    p.dw = dw->data_ptr<float>();
+  }
+  flare::combine_backward(p, stream());
+  return {dz, dw};
+}
+
+void fill(flare::GroupedArgs& a, const Tensor& offsets, const Tensor& like, int64_t G, int64_t status, int64_t timeout_ns) {
+  a.offsets = ints(offsets, like, G + 1, "offsets");
+  a.G = static_cast<int>(G);
+  a.status = reinterpret_cast<int*>(status);
+  a.timeout_ns = static_cast<uint64_t>(timeout_ns);
+}
+
+// y [R, N]: rows of x (or x[rows]) times their group's weight [G, K, N], plus its bias
+Tensor grouped_forward(const Tensor& x, const Tensor& w, const optional<Tensor>& bias, const Tensor& offsets, const optional<Tensor>& rows,
+                       int64_t status, int64_t timeout_ns) {
+  check_rows(x, "grouped_linear");
+  const c10::cuda::CUDAGuard guard(x.device());
+  TORCH_CHECK(w.dim() == 3 && w.is_contiguous() && w.scalar_type() == x.scalar_type() && w.device() == x.device() && w.size(1) == x.size(1),
+              "grouped_linear: weight [groups, in, out] of x's type");
+  flare::GroupedArgs a{};
+  a.mode = flare::kGroupedFwd;
+  a.dtype = code_of(x.scalar_type());
+  a.x = x.data_ptr();
+  a.ldx = pitch(x);
+  a.x_rows = x.size(0);
+  a.R = rows.has_value() ? rows->numel() : x.size(0);
+  if (rows.has_value()) a.rows = ints(*rows, x, a.R, "rows");
+  a.w = w.data_ptr();
+  a.K = static_cast<int>(w.size(1));
+  a.N = static_cast<int>(w.size(2));
+  fill(a, offsets, x, w.size(0), status, timeout_ns);
+  if (bias.has_value()) {
+    TORCH_CHECK(bias->is_contiguous() && bias->numel() == w.size(0) * w.size(2) && bias->device() == x.device(), "grouped_linear: bias [groups, out]");
+    a.bias = bias->data_ptr();
+    a.bias_dtype = code_of(bias->scalar_type());
+  }
+  Tensor y = empty({a.R, w.size(2)}, x, x.scalar_type());
+  if (a.x_rows == 0 || a.R == 0) return y.zero_();
+  a.out = y.data_ptr();
+  a.out_dtype = a.dtype;
+  flare::grouped_gemm(a, stream());
+  return y;
+}
+
+// dX of the rows [R, K], in dy's type or float32
+Tensor grouped_input_grad(const Tensor& dy, const Tensor& w, const Tensor& offsets, at::ScalarType out, int64_t status, int64_t timeout_ns) {
+  check_rows(dy, "grouped_linear gradient");
+  const c10::cuda::CUDAGuard guard(dy.device());
+  TORCH_CHECK(w.dim() == 3 && w.is_contiguous() && w.scalar_type() == dy.scalar_type() && w.device() == dy.device() && w.size(2) == dy.size(1),
+              "grouped_linear: gradient of another size or type");
+  flare::GroupedArgs a{};
+  a.mode = flare::kGroupedDgrad;
+  a.dtype = code_of(dy.scalar_type());
+  a.dy = dy.data_ptr();
+  a.lddy = pitch(dy);
+  a.R = dy.size(0);
+  a.w = w.data_ptr();
+  a.K = static_cast<int>(w.size(1));
+  a.N = static_cast<int>(w.size(2));
+  fill(a, offsets, dy, w.size(0), status, timeout_ns);
+  Tensor dx = empty({a.R, w.size(1)}, dy, out);
+  if (a.R == 0) return dx;
+  a.out = dx.data_ptr();
+  a.out_dtype = code_of(out);
+  flare::grouped_gemm(a, stream());
+  return dx;
+}
+
+// dW [G, K, N] and db [G, N], where they are given: written, or (fp32 only) added to
+void grouped_weight_grad(const Tensor& x, const Tensor& dy, const Tensor& offsets, const optional<Tensor>& rows, const optional<Tensor>& dw,
+                         bool accumulate, const optional<Tensor>& db, bool accumulate_bias, int64_t G, int64_t status, int64_t timeout_ns) {
+  check_rows(x, "grouped_linear");
+  check_rows(dy, "grouped_linear gradient");
+  const c10::cuda::CUDAGuard guard(x.device());
+  TORCH_CHECK(x.scalar_type() == dy.scalar_type() && x.device() == dy.device(), "grouped_linear: type of the gradient");
+  flare::GroupedArgs a{};
+  a.mode = flare::kGroupedWgrad;
+  a.dtype = code_of(x.scalar_type());
+  a.x = x.data_ptr();
+  a.ldx = pitch(x);
+  a.x_rows = x.size(0);
+  a.dy = dy.data_ptr();
+  a.lddy = pitch(dy);
+  a.R = dy.size(0);
+  if (rows.has_value()) a.rows = ints(*rows, x, a.R, "rows");
+  else TORCH_CHECK(x.size(0) == a.R, "grouped_linear: gradient of another size");
+  a.K = static_cast<int>(x.size(1));
+  a.N = static_cast<int>(dy.size(1));
+  fill(a, offsets, x, G, status, timeout_ns);
+  const bool none = a.x_rows == 0 || a.R == 0;
+  if (dw.has_value()) {
+    TORCH_CHECK(dw->is_contiguous() && dw->device() == x.device() && dw->numel() == G * x.size(1) * dy.size(1) &&
+                    (!accumulate || dw->scalar_type() == at::kFloat),
+                "grouped_linear: weight gradient [groups, in, out], accumulated in float32");
+    if (none && !accumulate) dw->zero_();
+    a.out = dw->data_ptr();
+    a.out_dtype = code_of(dw->scalar_type());
+    a.accumulate = accumulate ? 1 : 0;
+    if (!none) flare::grouped_gemm(a, stream());
+  }
+  if (db.has_value()) {
+    TORCH_CHECK(db->is_contiguous() && db->device() == x.device() && db->numel() == G * dy.size(1) &&
+                    (!accumulate_bias || db->scalar_type() == at::kFloat),
+                "grouped_linear: bias gradient [groups, out], accumulated in float32");
+    if (none && !accumulate_bias) db->zero_();
+    flare::GroupSumArgs b{};
+    b.y = a.dy;
+    b.ldy = a.lddy;
+    b.R = a.R;
+    b.dtype = a.dtype;
+    b.offsets = a.offsets;
+    b.G = a.G;
+    b.N = a.N;
+    b.out = db->data_ptr();
+    b.out_dtype = code_of(db->scalar_type());
+    b.accumulate = accumulate_bias ? 1 : 0;
+    if (!none) flare::group_colsum(b, stream());
+  }
+}
+
+// ------------------------------------------------------------ graph nodes
+void once(const char* what) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), what, " has no second derivative");
+}
+bool wants(std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : ts)
+    if (t->requires_grad()) return true;
+  return false;
+}
+optional<Tensor> some(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : std::nullopt; }
+Tensor unit_rows(const Tensor& t) { return t.stride(1) == 1 || t.size(1) <= 1 ? t : t.contiguous(); }
+
+// Rows that the tiled loads can address: unit inner stride, 16-byte aligned rows.  Others are copied.
+Tensor tma_rows(const Tensor& t) {
+  const bool aligned = reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  if (aligned && t.stride(1) == 1 && (t.size(0) <= 1 || (t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1)))) return t;
+  return t.is_contiguous() ? t.clone() : t.contiguous();
+}
+
+struct RouteFn : torch::autograd::Function<RouteFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, int64_t k) {
+    auto [experts, weights, offsets, rows, row_of] = route_topk(logits, k);
+    ctx->save_for_backward({experts, weights});
+    ctx->saved_data["n"] = logits.size(2);
+    ctx->saved_data["type"] = static_cast<int64_t>(logits.scalar_type());
+    ctx->mark_non_differentiable({experts, offsets, rows, row_of});
+    return {experts, weights, offsets, rows, row_of};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    once("route_topk");
+    const auto saved = ctx->get_saved_variables();
+    if (!g[1].defined()) return {Tensor(), Tensor()};
+    return {route_topk_backward(saved[0], saved[1], g[1].to(at::kFloat).contiguous(), ctx->saved_data["n"].toInt(),
+                                static_cast<at::ScalarType>(ctx->saved_data["type"].toInt())),
+            Tensor()};
+  }
+};
+
+struct SwigluFn : torch::autograd::Function<SwigluFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, bool keep) {
+    auto [y, q, scale] = swiglu_forward(x, keep);
+    if (keep) ctx->save_for_backward({q, scale});
+    else ctx->save_for_backward({x});
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    once("swiglu");
+    const auto saved = ctx->get_saved_variables();
+    if (!g[0].defined()) return {Tensor(), Tensor()};
+    const Tensor dy = unit_rows(g[0]);
+    return {saved.size() == 2 ? swiglu_backward(std::nullopt, saved[0], saved[1], dy) : swiglu_backward(saved[0], std::nullopt, std::nullopt, dy),
+            Tensor()};
+  }
+};
+
+struct CombineFn : torch::autograd::Function<CombineFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& z, const optional<Tensor>& weights, const Tensor& offsets, const Tensor& row_of) {
+    const int64_t k = row_of.size(-1);
+    Tensor y = combine_forward(z, row_of, weights, row_of.numel() / k, k, z.scalar_type());
+    ctx->save_for_backward({weights.has_value() ? z : Tensor(), weights.value_or(Tensor()), offsets, row_of});
+    ctx->saved_data["R"] = z.size(0);
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    once("combine_rows");
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &z = saved[0], &weights = saved[1], &offsets = saved[2], &row_of = saved[3];
+    if (!g[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    const int64_t k = row_of.size(-1);
+    auto [dz, dw] = combine_backward(some(z), row_of, some(weights), offsets, unit_rows(g[0]), ctx->saved_data["R"].toInt(), row_of.numel() / k, k);
+    return {dz, dw.has_value() ? dw->view(weights.sizes()) : Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// A weight (or bias) bound to a flat fused optimizer (flat_w, flat_b: its fp32 view of the gradient
+// buffer) gets its gradient added there by the kernel; others get a gradient of their own type.
+struct GroupedLinearFn : torch::autograd::Function<GroupedLinearFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const optional<Tensor>& bias, const Tensor& offsets,
+                        const optional<Tensor>& rows, const optional<Tensor>& row_of, const optional<Tensor>& flat_w,
+                        const optional<Tensor>& flat_b, const Tensor& w, int64_t status, int64_t timeout_ns) {
+    Tensor y = grouped_forward(x, w, bias, offsets, rows, status, timeout_ns);
+    ctx->save_for_backward({x, w, offsets, rows.value_or(Tensor()), row_of.value_or(Tensor())});
+    ctx->saved_data["flat_w"] = flat_w;
+    ctx->saved_data["flat_b"] = flat_b;
+    ctx->saved_data["wshape"] = weight.sizes();
+    ctx->saved_data["wtype"] = static_cast<int64_t>(weight.scalar_type());
+    if (bias.has_value()) {
+      ctx->saved_data["bshape"] = bias->sizes();
+      ctx->saved_data["btype"] = static_cast<int64_t>(bias->scalar_type());
+    }
+    ctx->saved_data["x?"] = x.requires_grad();
+    ctx->saved_data["w?"] = weight.requires_grad();
+    ctx->saved_data["b?"] = bias.has_value() && bias->requires_grad();
+    ctx->saved_data["status"] = status;
+    ctx->saved_data["timeout"] = timeout_ns;
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    once("grouped_linear");
+    variable_list out(11);
+    if (!g[0].defined()) return out;
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &w = saved[1], &offsets = saved[2], &rows = saved[3], &row_of = saved[4];
+    auto& d = ctx->saved_data;
+    const int64_t status = d["status"].toInt(), timeout = d["timeout"].toInt();
+    const Tensor dy = tma_rows(g[0]);
+    if (d["x?"].toBool() && ctx->needs_input_grad(0)) {
+      if (rows.defined()) {  // a token's gradient is the sum over its rows: kept in fp32 until it is complete
+        const Tensor dr = grouped_input_grad(dy, w, offsets, at::kFloat, status, timeout);
+        out[0] = combine_forward(dr, row_of, std::nullopt, x.size(0), row_of.size(-1), x.scalar_type());
+      } else {
+        out[0] = grouped_input_grad(dy, w, offsets, x.scalar_type(), status, timeout);
+      }
+    }
+    const bool need_w = d["w?"].toBool() && ctx->needs_input_grad(1), need_b = d["b?"].toBool() && ctx->needs_input_grad(2);
+    if (!need_w && !need_b) return out;
+    const optional<Tensor> flat_w = d["flat_w"].toOptional<Tensor>(), flat_b = d["flat_b"].toOptional<Tensor>();
+    Tensor dw, db;
+    if (need_w) dw = flat_w.has_value() ? flat_w->view(w.sizes()) : empty(w.sizes(), w, static_cast<at::ScalarType>(d["wtype"].toInt()));
+    if (need_b) db = flat_b.has_value() ? flat_b->view({-1}) : empty(d["bshape"].toIntVector(), w, static_cast<at::ScalarType>(d["btype"].toInt()));
+    grouped_weight_grad(x, dy, offsets, some(rows), some(dw), flat_w.has_value(), some(db), flat_b.has_value(), w.size(0), status, timeout);
+    if (need_w && !flat_w.has_value()) out[1] = dw.view(d["wshape"].toIntVector());
+    if (need_b && !flat_b.has_value()) out[2] = db;
+    return out;
+  }
+};
+
+// ------------------------------------------------------------ entry points
+py::tuple route_topk_op(const Tensor& logits, int64_t k) {
+  if (wants({&logits})) {
+    const auto o = RouteFn::apply(logits, k);
+    return py::make_tuple(o[0], o[1], o[2], o[3], o[4]);
+  }
+  const auto [experts, weights, offsets, rows, row_of] = route_topk(logits, k);
+  return py::make_tuple(experts, weights, offsets, rows, row_of);
+}
+
+Tensor swiglu_op(const Tensor& x, bool keep) {
+  const Tensor v = unit_rows(x);
+  if (wants({&v})) return SwigluFn::apply(v, keep);
+  return std::get<0>(swiglu_forward(v, false));
+}
+
+Tensor combine_rows_op(const Tensor& z, const optional<Tensor>& weights, const Tensor& offsets, const Tensor& row_of) {
+  const Tensor v = unit_rows(z);
+  optional<Tensor> w;
+  if (weights.has_value()) w = weights->to(at::kFloat).contiguous();
+  if (wants({&v}) || (w.has_value() && wants({&*w}))) return CombineFn::apply(v, w, offsets, row_of);
+  const int64_t k = row_of.size(-1);
+  return combine_forward(v, row_of, w, row_of.numel() / k, k, v.scalar_type());
+}
+
+Tensor grouped_linear_op(const Tensor& x, const Tensor& weight, const optional<Tensor>& bias, const Tensor& offsets, const optional<Tensor>& rows,
+                         const optional<Tensor>& row_of, const optional<Tensor>& flat_w, const optional<Tensor>& flat_b, int64_t status,
+                         int64_t timeout_ns) {
+  const Tensor v = tma_rows(x);
+  optional<Tensor> b;
+  if (bias.has_value()) b = bias->contiguous();
+  Tensor w = weight.detach().reshape({-1, weight.size(-2), weight.size(-1)}).to(x.scalar_type()).contiguous();
+  if (reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 != 0) w = w.clone();
+  if (wants({&v, &weight}) || (b.has_value() && wants({&*b})))
+    return GroupedLinearFn::apply(v, weight, b, offsets, rows, row_of, flat_w, flat_b, w, status, timeout_ns);
+  return grouped_forward(v, w, b, offsets, rows, status, timeout_ns);
+}
+
+}  // namespace
+
+void register_experts(py::module_& m) {
+  m.def("route_topk", &route_topk_op);
+  m.def("swiglu", &swiglu_op);
+  m.def("combine_rows", &combine_rows_op);
+  m.def("grouped_linear", &grouped_linear_op);
+}

@@ -5,7 +5,7 @@ Same constructor contracts and semantics as the reference's layer library
 (side-information tables grouped by dim, sum/mean pooling with id 0 as null,
 fp32 tables); the multitask gates ``PLE`` / ``CGC`` / ``UPLE`` / ``UCGC``;
 ``TokenMix``; ``BatchedExpertMoE`` (dense or top-k soft gating, SwiGLU
-experts, RMS-normalised residual); the multi-head MoE token mixers
+experts, RMS-normalised residual; routed, it computes the chosen experts only); the multi-head MoE token mixers
 ``TokenMixLargeMoe`` / ``TokenMixLargePreGateNoPool``; ``NamedTokens``; fp32
 numerics helpers.
 
@@ -28,6 +28,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from ..ops.dense import colsum_
+from ..ops.experts import expert_mlp
 from ..ops.gemm import gemm
 from ..ops.mixing import gate_mix, relu_bwd_colsum_
 
@@ -456,12 +457,20 @@ class TokenMix(nn.Module):
 class BatchedExpertMoE(nn.Module):
     """Per-slot batched SwiGLU experts with dense or top-k softmax gating.
 
-    Input ``x`` is [slots, batch, in_dim]; every slot has its own experts.
+    Input ``x`` is [slots, batch, in_dim]; every slot has its own experts.  ``routed`` (with ``sparse``) computes
+    only the chosen experts of every token (``ops.experts.expert_mlp``: routing, grouped products, combination) instead
+    of all of them; on CUDA x is then bf16 or fp16.  ``checkpoint="e4m3"`` (with ``routed``) keeps the experts' input
+    activations in 8 bits for the backward pass.
     """
 
     def __init__(self, batch_dim: int, in_dim: int, scale_size: int, num_experts: int, sparse: bool, top_k: int,
-                 residual_norm: bool = True):
+                 residual_norm: bool = True, routed: bool = False, checkpoint: str | None = None):
         super().__init__()
+        if routed and not sparse:
+            raise ValueError("routed experts need sparse gating")
+        if checkpoint is not None and not routed:
+            raise ValueError("checkpoint is an option of routed experts")
+        self.routed, self.checkpoint = routed, checkpoint
         self.batch_dim, self.in_dim, self.num_experts = batch_dim, in_dim, num_experts
         self.sparse, self.top_k, self.residual_norm = sparse, min(top_k, num_experts), residual_norm
         h = in_dim * scale_size
@@ -475,7 +484,17 @@ class BatchedExpertMoE(nn.Module):
         self.b_down = nn.Parameter(torch.zeros(batch_dim, num_experts, in_dim))
         self.norm_scale = nn.Parameter(torch.ones(batch_dim, in_dim))
 
+    def _forward_routed(self, x: torch.Tensor) -> torch.Tensor:
+        logits = torch.einsum("dbi,dio->dbo", x, self.w_gate.to(x.dtype)) + self.b_gate.to(x.dtype).unsqueeze(1)
+        moe = expert_mlp(x, logits, self.w_up, self.b_up, self.w_down, self.b_down, top_k=self.top_k,
+                         checkpoint=self.checkpoint)
+        if self.residual_norm:
+            return (fp32_rms_normalize(x + moe, -1) * self.norm_scale.unsqueeze(1)).to(x.dtype)
+        return moe
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if self.routed and self.num_experts > 1:
+            return self._forward_routed(x)
         up_gate = torch.einsum("dbi,deih->dbeh", x, self.w_up) + self.b_up.unsqueeze(1)
         up, gate = up_gate.chunk(2, -1)
         hidden = F.silu(gate) * up
@@ -530,16 +549,18 @@ class TokenMixLargeMoe(nn.Module):
     """
 
     def __init__(self, layer_num: int, token_num: int, token_dim: int, head_num: int = 12, scale_size: int = 4,
-                 num_experts: int = 1, sparse: bool = False, top_k: int = 2):
+                 num_experts: int = 1, sparse: bool = False, top_k: int = 2, routed: bool = False,
+                 checkpoint: str | None = None):
         super().__init__()
         if token_dim % head_num:
             raise ValueError(f"token_dim {token_dim} must be divisible by head_num {head_num}")
         self.layer_num, self.token_num, self.token_dim, self.head_num = layer_num, token_num, token_dim, head_num
         self.head_dim = token_dim // head_num
         k = min(top_k, num_experts)
+        how = dict(routed=routed, checkpoint=checkpoint)
         self.head_moe = nn.ModuleList(BatchedExpertMoE(head_num, token_num * self.head_dim, scale_size, num_experts,
-                                                       sparse, k) for _ in range(layer_num))
-        self.token_moe = nn.ModuleList(BatchedExpertMoE(token_num, token_dim, scale_size, num_experts, sparse, k)
+                                                       sparse, k, **how) for _ in range(layer_num))
+        self.token_moe = nn.ModuleList(BatchedExpertMoE(token_num, token_dim, scale_size, num_experts, sparse, k, **how)
                                        for _ in range(layer_num))
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
@@ -561,7 +582,7 @@ class TokenMixLargePreGateNoPool(nn.Module):
 
     def __init__(self, layer_num: int, token_num: int, token_dim: int, head_num: int = 12, scale_size: int = 4,
                  num_experts: int = 1, sparse: bool = False, top_k: int = 2, residual_enabled: bool = False,
-                 residual_layers: Sequence[int] = ()):
+                 residual_layers: Sequence[int] = (), routed: bool = False, checkpoint: str | None = None):
         super().__init__()
         if token_dim % head_num:
             raise ValueError(f"token_dim {token_dim} must be divisible by head_num {head_num}")
@@ -573,10 +594,11 @@ class TokenMixLargePreGateNoPool(nn.Module):
         self.residual_enabled, self.residual_layers = residual_enabled, frozenset(residual_layers)
         k = min(top_k, num_experts)
         hw = token_num * self.head_dim
-        self.head_moe = nn.ModuleList(BatchedExpertMoE(head_num, hw, scale_size, num_experts, sparse, k,
-                                                       residual_norm=False) for _ in range(layer_num))
-        self.token_moe = nn.ModuleList(BatchedExpertMoE(token_num, token_dim, scale_size, num_experts, sparse, k,
-                                                        residual_norm=False) for _ in range(layer_num))
+        how = dict(residual_norm=False, routed=routed, checkpoint=checkpoint)
+        self.head_moe = nn.ModuleList(BatchedExpertMoE(head_num, hw, scale_size, num_experts, sparse, k, **how)
+                                      for _ in range(layer_num))
+        self.token_moe = nn.ModuleList(BatchedExpertMoE(token_num, token_dim, scale_size, num_experts, sparse, k, **how)
+                                       for _ in range(layer_num))
         self.head_norms = nn.ModuleList(RMSNorm(hw) for _ in range(layer_num))
         self.token_norms = nn.ModuleList(RMSNorm(token_dim) for _ in range(layer_num))
         self.block_norms = nn.ModuleDict({str(i): RMSNorm(token_dim) for i in sorted(self.residual_layers)})

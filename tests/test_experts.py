@@ -1,0 +1,223 @@
+"""Routed experts on the CPU: the plain forms against the definitions, the layers that use them, and the refusals
+that need no device."""
+import math
+
+import pytest
+import torch
+
+from flare_b200.models.layers import BatchedExpertMoE, TokenMixLargeMoe, TokenMixLargePreGateNoPool
+from flare_b200.ops.experts import (ExpertRoute, combine_rows, e4m3_checkpoint_reference, expert_mlp, grouped_linear, route_topk,
+                                    swiglu)
+
+
+def _loop_route(logits, k):
+    """Token by token, in Python numbers."""
+    S, B, E = logits.shape
+    chosen, rows = {}, {}
+    for s in range(S):
+        for b in range(B):
+            lg = [float(v) for v in logits[s, b]]
+            order = sorted(range(E), key=lambda e: (-lg[e] if not math.isnan(lg[e]) else -math.inf, e))
+            order = sorted(order, key=lambda e: 0 if math.isnan(lg[e]) else 1)
+            chosen[s, b] = [e for e in order[:k] if lg[e] != -math.inf]
+    r, offsets = 0, [0]
+    for s in range(S):
+        for e in range(E):
+            for b in range(B):
+                if e in chosen[s, b]:
+                    rows[r] = (s * B + b, chosen[s, b].index(e))
+                    r += 1
+            offsets.append(r)
+    return chosen, rows, offsets
+
+
+def check_route(route, logits, k):
+    """A route's whole numbers against the loop."""
+    S, B, E = logits.shape
+    chosen, rows, offsets = _loop_route(logits, k)
+    experts, row_of = route.experts.view(S, B, k).tolist(), route.row_of.view(S * B, k).tolist()
+    for (s, b), c in chosen.items():
+        assert experts[s][b] == c + [-1] * (k - len(c))
+    assert route.offsets.tolist() == offsets
+    assert route.rows.tolist() == [rows[r][0] for r in range(len(rows))] + [-1] * (S * B * k - len(rows))
+    for r, (t, j) in rows.items():
+        assert row_of[t][j] == r
+    assert sum(v >= 0 for line in row_of for v in line) == len(rows)
+
+
+def hard_logits(S, B, E, seed, dtype=torch.float32):
+    """Ties, masked experts, tokens with nothing left, signed zeros."""
+    gen = torch.Generator().manual_seed(seed)
+    lg = torch.randint(-3, 4, (S, B, E), generator=gen).float() * 0.5
+    lg[torch.rand(S, B, E, generator=gen) < 0.3] = -math.inf
+    lg[torch.rand(S, B, E, generator=gen) < 0.1] = -0.0
+    lg[:, B // 2] = -math.inf
+    return lg.to(dtype)
+
+
+@pytest.mark.parametrize("S,B,E,k", [(1, 1, 1, 1), (1, 9, 4, 4), (3, 7, 5, 2), (2, 20, 33, 3)])
+def test_route_reference(S, B, E, k):
+    lg = hard_logits(S, B, E, S + B + E)
+    route = route_topk(lg, k)
+    check_route(route, lg, k)
+    w = route.weights
+    live = route.experts >= 0
+    assert torch.equal(w == 0, ~live)
+    torch.testing.assert_close(w.sum(-1), live.any(-1).float(), rtol=0, atol=k * 2 ** -23)
+    assert torch.equal(route_topk(lg[0], k).experts, route_topk(lg[:1], k).experts[0])
+
+
+def test_route_nan_is_largest():
+    lg = torch.tensor([[[0.0, math.nan, 3.0, math.inf]]])
+    route = route_topk(lg, 2)
+    assert route.experts.tolist() == [[[1, 3]]] and route.weights.isnan().all()
+
+
+def test_route_gradient_by_differences():
+    torch.manual_seed(0)
+    lg = torch.randn(2, 5, 6, dtype=torch.float64)
+    lg[0, 1, 2] = -math.inf
+    lg[1, 3] = -math.inf
+    finite = torch.isfinite(lg)
+    g = torch.randn(2, 5, 3, dtype=torch.float64)
+    x = lg.clone().requires_grad_(True)
+    (route_topk(x, 3).weights * g).sum().backward()
+    h = 1e-6
+    for i in finite.nonzero().tolist():
+        up, dn = lg.clone(), lg.clone()
+        up[tuple(i)] += h
+        dn[tuple(i)] -= h
+        d = ((route_topk(up, 3).weights - route_topk(dn, 3).weights) * g).sum() / (2 * h)
+        assert abs(float(d) - float(x.grad[tuple(i)])) < 1e-7  # h^2 and 64-bit rounding over 2h
+    assert torch.equal(x.grad[~finite], torch.zeros_like(x.grad[~finite]))
+
+
+def test_grouped_linear_reference_rows_outside_groups():
+    torch.manual_seed(1)
+    x, w, b = torch.randn(10, 3), torch.randn(3, 3, 2), torch.randn(3, 2)
+    y = grouped_linear(x, w, b, offsets=torch.tensor([2, 5, 5, 9], dtype=torch.int32))
+    want = torch.zeros(10, 2)
+    want[2:5] = x[2:5] @ w[0] + b[0]
+    want[5:9] = x[5:9] @ w[2] + b[2]
+    torch.testing.assert_close(y, want)
+
+
+def test_checkpoint_values():
+    """Every value of a group lands on an e4m3 value times the group's power of two, nearest to it."""
+    grid = torch.tensor([m * 2.0 ** e / 8 for e in range(-6, 9) for m in range(8, 16)] + [m * 2.0 ** -9 for m in range(8)])
+    grid = grid[grid <= 448]
+    torch.manual_seed(2)
+    x = torch.randn(6, 2 * 37) * torch.exp(3 * torch.randn(6, 1))
+    q = e4m3_checkpoint_reference(x)
+    for half in (slice(0, 37), slice(37, 74)):
+        for c in (0, 32):
+            v, got = x[:, half][:, c:c + 32], q[:, half][:, c:c + 32]
+            top = v.abs().amax(1, keepdim=True)
+            scale = 2.0 ** torch.ceil(torch.log2(top / 448))
+            near = (v / scale).abs().unsqueeze(-1).sub(grid).abs().amin(-1)
+            on_grid = (got / scale).abs().unsqueeze(-1).sub(grid).abs().amin(-1)
+            assert torch.equal(on_grid, torch.zeros_like(on_grid))
+            torch.testing.assert_close((got / scale - v / scale).abs(), near, rtol=0, atol=1e-4)
+
+
+def test_checkpoint_keeps_other_values_beside_infinities():
+    x = torch.ones(1, 64)
+    x[0, 3], x[0, 40], x[0, 5] = math.inf, math.nan, 0.0
+    q = e4m3_checkpoint_reference(x)
+    assert q.isnan().nonzero().tolist() == [[0, 3], [0, 40]]
+    ok = ~q.isnan()
+    assert torch.equal(q[ok], x[ok])
+
+
+def test_swiglu_gradient_is_the_formula_at_the_checkpoint():
+    torch.manual_seed(3)
+    x = torch.randn(5, 20, dtype=torch.float64)
+    g = torch.randn(5, 10, dtype=torch.float64)
+    for checkpoint in (None, "e4m3"):
+        leaf = x.clone().requires_grad_(True)
+        swiglu(leaf, checkpoint=checkpoint).backward(g)
+        at = (e4m3_checkpoint_reference(x).double() if checkpoint else x.clone()).requires_grad_(True)
+        (at[:, :10] * torch.nn.functional.silu(at[:, 10:])).backward(g)
+        torch.testing.assert_close(leaf.grad, at.grad)
+
+
+@pytest.mark.parametrize("slots", [1, 3])
+def test_expert_mlp_matches_all_experts_then_pick(slots):
+    """The routed block against the sparse layer that computes every expert, outputs and gradients, in 64 bits."""
+    torch.manual_seed(4)
+    dense = BatchedExpertMoE(slots, 6, 2, 5, True, 2).double()
+    routed = BatchedExpertMoE(slots, 6, 2, 5, True, 2, routed=True).double()
+    with torch.no_grad():
+        for p in dense.parameters():
+            p.add_(0.1 * torch.randn_like(p))
+    routed.load_state_dict(dense.state_dict())
+    x = torch.randn(slots, 11, 6, dtype=torch.float64)
+    xs = [x.clone().requires_grad_(True) for _ in range(2)]
+    ys = [m(v) for m, v in zip((dense, routed), xs)]
+    g = torch.randn_like(ys[0])
+    for y in ys:
+        y.backward(g)
+    # the routed layer's norm is of the same formula; softmax weights are 32-bit in the dense layer
+    torch.testing.assert_close(ys[1], ys[0], rtol=1e-5, atol=1e-6)
+    torch.testing.assert_close(xs[1].grad, xs[0].grad, rtol=1e-4, atol=1e-5)
+    for (n, p), (_, q) in zip(routed.named_parameters(), dense.named_parameters()):
+        torch.testing.assert_close(p.grad, q.grad, rtol=1e-4, atol=1e-5, msg=n)
+
+
+def test_token_mixers_pass_the_option_on():
+    torch.manual_seed(5)
+    x = torch.randn(4, 4, 24)
+    for cls in (TokenMixLargeMoe, TokenMixLargePreGateNoPool):
+        a = cls(2, 4, 24, head_num=6, scale_size=2, num_experts=3, sparse=True, top_k=2)
+        b = cls(2, 4, 24, head_num=6, scale_size=2, num_experts=3, sparse=True, top_k=2, routed=True, checkpoint="e4m3")
+        b.load_state_dict(a.state_dict())
+        assert all(m.routed and m.checkpoint == "e4m3" for m in b.modules() if isinstance(m, BatchedExpertMoE))
+        torch.testing.assert_close(b(x), a(x), rtol=1e-4, atol=1e-5)
+
+
+def test_no_tokens():
+    route = route_topk(torch.empty(2, 0, 3), 2)
+    assert route.offsets.tolist() == [0] * 7 and route.rows.numel() == 0
+    y = expert_mlp(torch.empty(2, 0, 4), torch.empty(2, 0, 3), torch.randn(2, 3, 4, 12), None, torch.randn(2, 3, 6, 4), None, top_k=2)
+    assert y.shape == (2, 0, 4)
+
+
+def test_refusals():
+    lg = torch.randn(4, 3)
+    with pytest.raises(ValueError, match="top_k"):
+        route_topk(lg, 4)
+    with pytest.raises(ValueError, match="top_k"):
+        route_topk(lg, 0)
+    with pytest.raises(ValueError, match="logits"):
+        route_topk(lg[0], 1)
+    route = route_topk(lg, 2)
+    x, w = torch.randn(4, 6), torch.randn(3, 6, 5)
+    with pytest.raises(ValueError, match="exactly one"):
+        grouped_linear(x, w)
+    with pytest.raises(ValueError, match="exactly one"):
+        grouped_linear(x, w, offsets=route.offsets, route=route)
+    with pytest.raises(ValueError, match="weight"):
+        grouped_linear(x, w.transpose(1, 2), route=route)
+    with pytest.raises(ValueError, match="offsets"):
+        grouped_linear(x, w[:2], route=route)
+    with pytest.raises(ValueError, match="offsets"):
+        grouped_linear(x, w, offsets=route.offsets.long())
+    with pytest.raises(ValueError, match="bias"):
+        grouped_linear(x, w, torch.randn(3, 6), route=route)
+    with pytest.raises(ValueError, match="tokens"):
+        grouped_linear(torch.randn(3, 6), w, route=route)
+    with pytest.raises(ValueError, match="2h"):
+        swiglu(torch.randn(3, 5))
+    with pytest.raises(ValueError, match="checkpoint"):
+        swiglu(torch.randn(3, 4), checkpoint="int4")
+    with pytest.raises(ValueError, match="route"):
+        combine_rows(torch.randn(7, 2), route)
+    with pytest.raises(ValueError, match="weights"):
+        combine_rows(torch.randn(8, 2), route, torch.randn(4, 3))
+    with pytest.raises(ValueError, match="same tokens"):
+        expert_mlp(x, lg[:3], w, None, w, None, top_k=2)
+    with pytest.raises(ValueError, match="sparse"):
+        BatchedExpertMoE(1, 4, 2, 3, False, 2, routed=True)
+    with pytest.raises(ValueError, match="routed"):
+        BatchedExpertMoE(1, 4, 2, 3, True, 2, checkpoint="e4m3")
+    assert ExpertRoute._fields == ("experts", "weights", "offsets", "rows", "row_of")
