@@ -25,20 +25,6 @@ namespace {
 // ------------------------------------------------------------------ routing
 constexpr int kSub = 256;  // tokens that are ranked together (one bit each)
 
-struct RouteShape {
-  int chunk_tokens;  // tokens of one block, a multiple of kSub
-  int chunks;        // blocks of one slot
-};
-
-// About two blocks per SM: every block of the second pass reads all blocks' counts, so their
-// number is bounded rather than their length.
-RouteShape route_shape(int S, int B) {
-  const int64_t per_slot = std::max<int64_t>(1, 296 / S);
-  int64_t tokens = (B + per_slot - 1) / per_slot;
-  tokens = std::max<int64_t>(kSub, (tokens + kSub - 1) / kSub * kSub);
-  return {static_cast<int>(tokens), static_cast<int>((B + tokens - 1) / tokens)};
-}
-
 // An unsigned key in the order of the logits: NaN above all, -0 equal to +0, -inf at kDeadKey.
 constexpr uint32_t kDeadKey = 0x007FFFFFu;
 __device__ __forceinline__ uint32_t order_key(float v) {
@@ -47,42 +33,53 @@ __device__ __forceinline__ uint32_t order_key(float v) {
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-// LANES lanes share a token, each with NV of its experts (expert = v * LANES + lane).
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? k & 0x7FFFFFFFu : ~k);
+}
+
+// LANES lanes share a token, each with NV of its experts (expert = v * LANES + lane); 0 is below
+// every logit's key.
 template <typename T, int LANES, int NV>
-__device__ __forceinline__ void route_pick(const RouteParams& p, int slot, int b, bool live_token, int* hist) {
+__device__ __forceinline__ void route_load(const RouteParams& p, int slot, int b, bool live, uint32_t (&key)[NV]) {
   const int sub = threadIdx.x % LANES;
   const T* row = static_cast<const T*>(p.logits) + slot * p.stride_slot + b * p.stride_token;
-  uint32_t key[NV];
-  float val[NV];
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     const int e = v * LANES + sub;
-    const bool in = live_token && e < p.E;
-    val[v] = in ? to_f32(row[e]) : -INFINITY;
-    key[v] = in ? order_key(val[v]) : 0u;
+    key[v] = live && e < p.E ? order_key(to_f32(row[e])) : 0u;
   }
+}
+
+template <int LANES, int NV>
+__device__ __forceinline__ void route_pick(const RouteParams& p, int slot, int b, bool live_token, uint32_t (&key)[NV],
+                                           int* hist) {
+  const int sub = threadIdx.x % LANES;
   int my_e = -1;  // lane j of the token keeps choice j
-  float my_v = -INFINITY;
+  uint32_t my_k = kDeadKey;
   for (int j = 0; j < p.k; ++j) {
     uint32_t best = 0;
     int at = 0;
-    float bv = -INFINITY;
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {  // the first of equal keys has the lowest expert
-      if (key[v] > best) best = key[v], at = v * LANES + sub, bv = val[v];
-    }
+    for (int v = 0; v < NV; ++v)  // the first of equal keys has the lowest expert
+      if (key[v] > best) best = key[v], at = v * LANES + sub;
+    if constexpr (LANES == 32) {
+      const uint32_t top = __reduce_max_sync(0xffffffffu, best);
+      at = __reduce_min_sync(0xffffffffu, best == top ? at : 0x7fffffff);
+      best = top;
+    } else {
 #pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) {
-      const uint32_t ob = __shfl_xor_sync(0xffffffffu, best, o);
-      const int oa = __shfl_xor_sync(0xffffffffu, at, o);
-      const float ov = __shfl_xor_sync(0xffffffffu, bv, o);
-      if (ob > best || (ob == best && oa < at)) best = ob, at = oa, bv = ov;
+      for (int o = LANES / 2; o > 0; o >>= 1) {
+        const uint32_t ob = __shfl_xor_sync(0xffffffffu, best, o);
+        const int oa = __shfl_xor_sync(0xffffffffu, at, o);
+        if (ob > best || (ob == best && oa < at)) best = ob, at = oa;
+      }
     }
-    if (sub == j && best > kDeadKey) my_e = at, my_v = bv;
+    if (sub == j && best > kDeadKey) my_e = at, my_k = best;
 #pragma unroll
     for (int v = 0; v < NV; ++v)
       if (v * LANES + sub == at) key[v] = 0u;
   }
+  const float my_v = key_value(my_k);
   const float top = __shfl_sync(0xffffffffu, my_v, 0, LANES);
   const float mine = my_e >= 0 ? expf(my_v - top) : 0.f;
   float sum = 0.f;
@@ -95,15 +92,21 @@ __device__ __forceinline__ void route_pick(const RouteParams& p, int slot, int b
   }
 }
 
-// The experts of tokens [b0, b1) of one slot; counts in hist[E] (shared memory, zeroed here).
+// The experts of tokens [b0, b1) of one slot; counts in hist[E] (shared memory, zeroed here).  The
+// next token's logits are on their way while a token is picked.
 template <typename T, int LANES, int NV>
 __device__ __forceinline__ void route_pick_chunk(const RouteParams& p, int slot, int b0, int b1, int* hist) {
   for (int e = threadIdx.x; e < p.E; e += blockDim.x) hist[e] = 0;
   __syncthreads();
-  const int per = blockDim.x / LANES;
+  const int per = blockDim.x / LANES, mine = b0 + threadIdx.x / LANES;
+  uint32_t key[NV], next[NV];
+  route_load<T, LANES, NV>(p, slot, mine, mine < b1, key);
   for (int b = b0; b < b1; b += per) {  // block-uniform: the picks shuffle across whole warps
-    const int mine = b + threadIdx.x / LANES;
-    route_pick<T, LANES, NV>(p, slot, min(mine, b1 - 1), mine < b1, hist);
+    const int at = mine + b - b0;
+    route_load<T, LANES, NV>(p, slot, at + per, at + per < b1, next);
+    route_pick<LANES, NV>(p, slot, at, at < b1, key, hist);
+#pragma unroll
+    for (int v = 0; v < NV; ++v) key[v] = next[v];
   }
   __syncthreads();
 }
@@ -162,62 +165,71 @@ __device__ __forceinline__ int warp_exclusive(int* tot, int E) {
   return carry;
 }
 
-// Pass 1: experts and weights of every token, and each block's counts: work[block][E + 1] (the
-// last entry is their sum).
+// Pass 1: experts and weights of every token of a sub-block (block = slot * chunks + chunk), and
+// its counts: work[slot][chunk][E].
 template <typename T, int LANES, int NV>
-__global__ void __launch_bounds__(256) route_pick_kernel(RouteParams p, RouteShape sh) {
+__global__ void __launch_bounds__(256) route_pick_kernel(RouteParams p, int chunks) {
   __shared__ int hist[kRouteMaxExperts];
-  __shared__ int sum;
-  const int slot = blockIdx.x / sh.chunks, c = blockIdx.x % sh.chunks;
-  if (threadIdx.x == 0) sum = 0;
-  route_pick_chunk<T, LANES, NV>(p, slot, c * sh.chunk_tokens, min(p.B, (c + 1) * sh.chunk_tokens), hist);
-  int* out = p.work + static_cast<int64_t>(blockIdx.x) * (p.E + 1);
-  int mine = 0;
-  for (int e = threadIdx.x; e < p.E; e += blockDim.x) out[e] = hist[e], mine += hist[e];
-  if (mine) atomicAdd(&sum, mine);
-  __syncthreads();
-  if (threadIdx.x == 0) out[p.E] = sum;
+  const int slot = blockIdx.x / chunks, c = blockIdx.x % chunks;
+  route_pick_chunk<T, LANES, NV>(p, slot, c * kSub, min(p.B, (c + 1) * kSub), hist);
+  int* out = p.work + static_cast<int64_t>(blockIdx.x) * p.E;
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) out[e] = hist[e];
 }
 
-// Pass 2: a block's first row of each expert = rows of the slots before + of the experts before
-// + of the blocks before; then its pairs' rows.
-__global__ void __launch_bounds__(256) route_place_kernel(RouteParams p, RouteShape sh) {
-  __shared__ int tot[kRouteMaxExperts], pre[kRouteMaxExperts];
+// Pass 2: along the chunks of a slot, counts become the rows of the same expert before the chunk;
+// their sum goes to work[S * chunks * E + group].  Block = 32 experts of a slot; thread y takes a
+// 32nd of the chunks.
+__global__ void __launch_bounds__(1024) route_scan_kernel(RouteParams p, int chunks) {
+  __shared__ int part[32][33];
+  const int e = blockIdx.y * 32 + threadIdx.x, slot = blockIdx.x;
+  const int per = (chunks + 31) / 32, q0 = min(chunks, static_cast<int>(threadIdx.y) * per), q1 = min(chunks, q0 + per);
+  int* col = p.work + static_cast<int64_t>(slot) * chunks * p.E + e;
+  int mine = 0;
+  if (e < p.E) {
+#pragma unroll 4
+    for (int q = q0; q < q1; ++q) mine += col[static_cast<int64_t>(q) * p.E];
+  }
+  part[threadIdx.y][threadIdx.x] = mine;
+  __syncthreads();
+  int run = 0;
+  for (int y = 0; y < static_cast<int>(threadIdx.y); ++y) run += part[y][threadIdx.x];
+  if (e >= p.E) return;
+#pragma unroll 4
+  for (int q = q0; q < q1; ++q) {
+    const int64_t i = static_cast<int64_t>(q) * p.E;
+    const int v = col[i];
+    col[i] = run;
+    run += v;
+  }
+  if (threadIdx.y == 31) p.work[(static_cast<int64_t>(p.S) * chunks + slot) * p.E + e] = run;
+}
+
+// Pass 3: a sub-block's first row of each expert = rows of the groups before + of the chunks
+// before; then its pairs' rows.
+__global__ void __launch_bounds__(256) route_place_kernel(RouteParams p, int chunks) {
+  __shared__ int base[kRouteMaxExperts];
   __shared__ uint32_t mask[kRouteMaxExperts * (kSub / 32)];
   __shared__ int before, total;
-  const int slot = blockIdx.x / sh.chunks, c = blockIdx.x % sh.chunks;
-  for (int e = threadIdx.x; e < p.E; e += blockDim.x) tot[e] = pre[e] = 0;
+  const int slot = blockIdx.x / chunks, c = blockIdx.x % chunks;
+  const int* counts = p.work + static_cast<int64_t>(p.S) * chunks * p.E;
   if (threadIdx.x == 0) before = total = 0;
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) base[e] = counts[slot * p.E + e];
   __syncthreads();
   int bsum = 0, tsum = 0;
-  for (int i = threadIdx.x; i < static_cast<int>(gridDim.x); i += blockDim.x) {
-    const int v = p.work[static_cast<int64_t>(i) * (p.E + 1) + p.E];
+  for (int i = threadIdx.x; i < p.S * p.E; i += blockDim.x) {
+    const int v = counts[i];
     tsum += v;
-    if (i / sh.chunks < slot) bsum += v;
+    if (i < slot * p.E) bsum += v;
   }
   if (bsum) atomicAdd(&before, bsum);
   if (tsum) atomicAdd(&total, tsum);
-  const int* mine = p.work + static_cast<int64_t>(slot) * sh.chunks * (p.E + 1);
-  // thread = expert where there are many, several blocks at a time where there are few
-  const int parts = max(1, static_cast<int>(blockDim.x) / p.E);
-  for (int i = threadIdx.x; i < parts * p.E; i += blockDim.x) {
-    const int e = i % p.E;
-    int a = 0, b = 0;
-    for (int q = i / p.E; q < sh.chunks; q += parts) {
-      const int v = mine[static_cast<int64_t>(q) * (p.E + 1) + e];
-      a += v;
-      if (q < c) b += v;
-    }
-    if (a) atomicAdd(&tot[e], a);
-    if (b) atomicAdd(&pre[e], b);
-  }
+  if (threadIdx.x < 32) warp_exclusive(base, p.E);
   __syncthreads();
-  if (threadIdx.x < 32) warp_exclusive(tot, p.E);
-  __syncthreads();
+  const int* mine = p.work + static_cast<int64_t>(blockIdx.x) * p.E;
   for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
-    const int first = before + tot[e];
+    const int first = before + base[e];
     if (c == 0) p.offsets[slot * p.E + e] = first;
-    pre[e] += first;
+    base[e] = first + mine[e];
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) p.offsets[p.S * p.E] = total;
   const int64_t R = static_cast<int64_t>(p.S) * p.B * p.k;
@@ -225,7 +237,7 @@ __global__ void __launch_bounds__(256) route_place_kernel(RouteParams p, RouteSh
        i += static_cast<int64_t>(gridDim.x) * blockDim.x)
     p.rows[i] = -1;
   __syncthreads();
-  route_place_chunk(p, slot, c * sh.chunk_tokens, min(p.B, (c + 1) * sh.chunk_tokens), pre, mask);
+  route_place_chunk(p, slot, c * kSub, min(p.B, (c + 1) * kSub), base, mask);
 }
 
 // Both passes in one block: one slot of at most kRouteOneBlock tokens.
@@ -258,43 +270,33 @@ void route_launch(const RouteParams& p, cudaStream_t s) {
     count_launch();
     return;
   }
-  const RouteShape sh = route_shape(p.S, p.B);
-  route_pick_kernel<T, LANES, NV><<<p.S * sh.chunks, 256, 0, s>>>(p, sh);
+  const int chunks = ceil_div(p.B, kSub);
+  route_pick_kernel<T, LANES, NV><<<p.S * chunks, 256, 0, s>>>(p, chunks);
   FLARE_CUDA_CHECK(cudaGetLastError());
-  route_place_kernel<<<p.S * sh.chunks, 256, 0, s>>>(p, sh);
+  route_scan_kernel<<<dim3(p.S, ceil_div(p.E, 32)), dim3(32, 32), 0, s>>>(p, chunks);
   FLARE_CUDA_CHECK(cudaGetLastError());
-  count_launch(2);
+  route_place_kernel<<<p.S * chunks, 256, 0, s>>>(p, chunks);
+  FLARE_CUDA_CHECK(cudaGetLastError());
+  count_launch(3);
 }
 
 template <typename T>
 void route_typed(const RouteParams& p, cudaStream_t s) {
-  if (p.E <= 8) route_launch<T, 8, 1>(p, s);
-  else if (p.E <= 16) route_launch<T, 16, 1>(p, s);
-  else if (p.E <= 32) route_launch<T, 32, 1>(p, s);
-  else if (p.E <= 64) route_launch<T, 32, 2>(p, s);
-  else if (p.E <= 128) route_launch<T, 32, 4>(p, s);
-  else if (p.E <= 256) route_launch<T, 32, 8>(p, s);
-  else route_launch<T, 32, 16>(p, s);
-}
-
-// d logits[t, e] = w_j (dw_j - sum_i w_i dw_i) where choice j of t is e, else 0.
-template <typename T>
-__global__ void __launch_bounds__(256) route_bwd_kernel(RouteBwdParams p, int lanes) {
-  const int sub = threadIdx.x % lanes;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * (blockDim.x / lanes);
-  for (int64_t t = static_cast<int64_t>(blockIdx.x) * (blockDim.x / lanes) + threadIdx.x / lanes; t < p.T; t += step) {
-    const int* ex = p.experts + t * p.k;
-    const float* w = p.weights + t * p.k;
-    const float* dw = p.dweights + t * p.k;
-    float dot = 0.f;
-    for (int j = 0; j < p.k; ++j) dot += ex[j] >= 0 ? w[j] * dw[j] : 0.f;
-    T* out = static_cast<T*>(p.dlogits) + t * p.E;
-    for (int e = sub; e < p.E; e += lanes) {
-      float g = 0.f;
-      for (int j = 0; j < p.k; ++j)
-        if (ex[j] == e) g = w[j] * (dw[j] - dot);
-      out[e] = from_f32<T>(g);
-    }
+  // Eight lanes a token where they can hold its choices: four tokens share each instruction
+  // (131071 x 128 fp32, k = 4: 97 us with 32 lanes a token).
+  if (p.k <= 8 && p.E <= 256) {
+    if (p.E <= 8) route_launch<T, 8, 1>(p, s);
+    else if (p.E <= 16) route_launch<T, 8, 2>(p, s);
+    else if (p.E <= 32) route_launch<T, 8, 4>(p, s);
+    else if (p.E <= 64) route_launch<T, 8, 8>(p, s);
+    else if (p.E <= 128) route_launch<T, 8, 16>(p, s);
+    else route_launch<T, 8, 32>(p, s);
+  } else if (p.E <= 64) {
+    route_launch<T, 32, 2>(p, s);
+  } else if (p.E <= 256) {
+    route_launch<T, 32, 8>(p, s);
+  } else {
+    route_launch<T, 32, 16>(p, s);
   }
 }
 
@@ -318,6 +320,56 @@ __device__ __forceinline__ void store_f(T* p, const float (&f)[N]) {
   *reinterpret_cast<Vec<T, N>*>(p) = u;
 }
 
+// d logits[t, e] = w_j (dw_j - sum_i w_i dw_i) where choice j of t is e, else 0.  A block takes
+// kBwdTokens tokens: a thread works out one token's k values, then all write the rows, which are
+// mostly zeros, in vectors of N.
+constexpr int kBwdTokens = 64;
+template <typename T, int N>
+__global__ void __launch_bounds__(256) route_bwd_kernel(RouteBwdParams p) {
+  extern __shared__ int ex[];  // [kBwdTokens][k], then the values
+  float* g = reinterpret_cast<float*>(ex + kBwdTokens * p.k);
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * kBwdTokens;
+  const int n = static_cast<int>(min(static_cast<long long>(kBwdTokens), static_cast<long long>(p.T - t0)));
+  for (int i = threadIdx.x; i < n * p.k; i += 256) {
+    ex[i] = p.experts[t0 * p.k + i];
+    g[i] = ex[i] >= 0 ? p.weights[t0 * p.k + i] * p.dweights[t0 * p.k + i] : 0.f;
+  }
+  __syncthreads();
+  if (threadIdx.x < n) {
+    const int i0 = threadIdx.x * p.k;
+    float dot = 0.f;
+    for (int j = 0; j < p.k; ++j) dot += g[i0 + j];
+    for (int j = 0; j < p.k; ++j) {
+      const int64_t i = t0 * p.k + i0 + j;
+      g[i0 + j] = ex[i0 + j] >= 0 ? p.weights[i] * (p.dweights[i] - dot) : 0.f;
+    }
+  }
+  __syncthreads();
+  const int per = p.E / N;
+  for (int c = threadIdx.x; c < n * per; c += 256) {
+    const int t = c / per, e0 = (c - t * per) * N;
+    float f[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = 0.f;
+    for (int j = 0; j < p.k; ++j) {
+      const int at = ex[t * p.k + j] - e0;
+      const float v = g[t * p.k + j];
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] = at == i ? v : f[i];
+    }
+    store_f<T, N>(static_cast<T*>(p.dlogits) + (t0 + t) * p.E + e0, f);
+  }
+}
+
+template <typename T, int N>
+void route_bwd_launch(const RouteBwdParams& p, cudaStream_t s) {
+  const int grid = static_cast<int>((p.T + kBwdTokens - 1) / kBwdTokens), smem = kBwdTokens * p.k * 8;
+  if (p.E % N == 0) route_bwd_kernel<T, N><<<grid, 256, smem, s>>>(p);
+  else route_bwd_kernel<T, 1><<<grid, 256, smem, s>>>(p);
+  FLARE_CUDA_CHECK(cudaGetLastError());
+  count_launch();
+}
+
 // ------------------------------------------------------------------ SwiGLU
 constexpr int kGroupCols = 32;
 
@@ -338,27 +390,56 @@ __device__ __forceinline__ int scale_exponent(float top) {
 }
 __device__ __forceinline__ float exp2_int(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
 
-__device__ __forceinline__ float finite_abs(float v) {
-  const float a = fabsf(v);
-  return a < INFINITY ? a : 0.f;  // NaN and infinities say nothing about the others
+// Largest finite magnitude of N values (NaN and infinities say nothing about the others); inf is
+// set where there is an infinity.
+template <int N>
+__device__ __forceinline__ float finite_top(const float (&v)[N], bool& inf) {
+  float t = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) t = fmaxf(t, fabsf(v[i]));  // fmaxf passes over NaN
+  inf = t == INFINITY;
+  if (inf) {
+    t = 0.f;
+    for (int i = 0; i < N; ++i) t = fmaxf(t, fabsf(v[i]) < INFINITY ? fabsf(v[i]) : 0.f);
+  }
+  return t;
 }
 
 // e4m3 of v * inv; infinities become NaN (e4m3 has no infinity), NaN stays.
 template <int N>
-__device__ __forceinline__ void pack_e4m3(const float (&v)[N], float inv, uint8_t* out) {
+__device__ __forceinline__ void pack_e4m3(const float (&v)[N], float inv, bool inf, uint8_t* out) {
   Vec<uint8_t, N> u;
+  if constexpr (N == 1) {
+    u.v[0] = static_cast<uint8_t>(__nv_cvt_float_to_fp8(v[0] * inv, __NV_SATFINITE, __NV_E4M3));
+  } else {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const bool inf = fabsf(v[i]) == INFINITY;
-    u.v[i] = inf ? 0x7F : static_cast<uint8_t>(__nv_cvt_float_to_fp8(v[i] * inv, __NV_SATFINITE, __NV_E4M3));
+    for (int i = 0; i < N; i += 2) {
+      const uint16_t two = __nv_cvt_float2_to_fp8x2(make_float2(v[i] * inv, v[i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+      u.v[i] = static_cast<uint8_t>(two & 0xFF);
+      u.v[i + 1] = static_cast<uint8_t>(two >> 8);
+    }
+  }
+  if (inf) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (fabsf(v[i]) == INFINITY) u.v[i] = 0x7F;
   }
   *reinterpret_cast<Vec<uint8_t, N>*>(out) = u;
 }
 template <int N>
 __device__ __forceinline__ void unpack_e4m3(const uint8_t* in, float scale, float (&v)[N]) {
   const Vec<uint8_t, N> u = *reinterpret_cast<const Vec<uint8_t, N>*>(in);
+  if constexpr (N == 1) {
+    v[0] = __half2float(__half(__nv_cvt_fp8_to_halfraw(u.v[0], __NV_E4M3))) * scale;
+  } else {
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = __half2float(__half(__nv_cvt_fp8_to_halfraw(u.v[i], __NV_E4M3))) * scale;
+    for (int i = 0; i < N; i += 2) {
+      const uint16_t two = static_cast<uint16_t>(u.v[i] | (u.v[i + 1] << 8));
+      const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3)));
+      v[i] = f.x * scale;
+      v[i + 1] = f.y * scale;
+    }
+  }
 }
 
 // A thread owns N consecutive columns of up and the same of gate; kGroupCols / N lanes share a
@@ -395,9 +476,8 @@ __global__ void __launch_bounds__(256) swiglu_fwd_kernel(SwigluParams p, RowTili
         store_f<T, N>(static_cast<T*>(p.y) + r * p.h + col, y);
       }
       if constexpr (kKeep) {
-        float tu = 0.f, tg = 0.f;
-#pragma unroll
-        for (int i = 0; i < N; ++i) tu = fmaxf(tu, finite_abs(up[i])), tg = fmaxf(tg, finite_abs(gate[i]));
+        bool iu, ig;
+        float tu = finite_top<N>(up, iu), tg = finite_top<N>(gate, ig);
 #pragma unroll
         for (int o = GL / 2; o > 0; o >>= 1) {
           tu = fmaxf(tu, __shfl_xor_sync(0xffffffffu, tu, o));
@@ -406,8 +486,8 @@ __global__ void __launch_bounds__(256) swiglu_fwd_kernel(SwigluParams p, RowTili
         if (in) {
           const int eu = scale_exponent(tu), eg = scale_exponent(tg);
           uint8_t* q = p.q + r * 2 * p.h + col;
-          pack_e4m3<N>(up, exp2_int(-eu), q);
-          pack_e4m3<N>(gate, exp2_int(-eg), q + p.h);
+          pack_e4m3<N>(up, exp2_int(-eu), iu, q);
+          pack_e4m3<N>(gate, exp2_int(-eg), ig, q + p.h);
           if (c % GL == 0) {
             uint8_t* sc = p.scale + r * 2 * groups + c / GL;
             sc[0] = static_cast<uint8_t>(eu + 127);
@@ -617,7 +697,7 @@ void combine_dispatch(const CombineParams& p, bool backward, cudaStream_t s) {
 
 int64_t route_work_ints(int S, int B, int E) {
   if (S == 1 && B <= kRouteOneBlock) return 0;
-  return static_cast<int64_t>(S) * route_shape(S, B).chunks * (E + 1);
+  return static_cast<int64_t>(S) * (ceil_div(B, kSub) + 1) * E;
 }
 
 void route_topk(const RouteParams& p, cudaStream_t s) {
@@ -633,15 +713,11 @@ void route_topk(const RouteParams& p, cudaStream_t s) {
 
 void route_topk_backward(const RouteBwdParams& p, cudaStream_t s) {
   if (p.T == 0) return;
-  const int lanes = p.E <= 8 ? 8 : p.E <= 16 ? 16 : 32;
-  const int grid = static_cast<int>(std::min<int64_t>((p.T + 256 / lanes - 1) / (256 / lanes), 148 * 16));
   switch (p.dtype) {
-    case kF32: route_bwd_kernel<float><<<grid, 256, 0, s>>>(p, lanes); break;
-    case kBF16: route_bwd_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(p, lanes); break;
-    default: route_bwd_kernel<__half><<<grid, 256, 0, s>>>(p, lanes); break;
+    case kF32: route_bwd_launch<float, 4>(p, s); break;
+    case kBF16: route_bwd_launch<__nv_bfloat16, 8>(p, s); break;
+    default: route_bwd_launch<__half, 8>(p, s); break;
   }
-  FLARE_CUDA_CHECK(cudaGetLastError());
-  count_launch();
 }
 
 void swiglu_forward(const SwigluParams& p, cudaStream_t s) { swiglu_dispatch(p, false, s); }

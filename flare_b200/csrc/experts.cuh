@@ -78,9 +78,9 @@ constexpr int kGroupedMaxGroups = 2048;
 struct GroupedArgs {
   int mode;
   int dtype;  // kBF16 or kF16: x, w, dy and (fwd, dgrad) out
-  const void* x;  // fwd, wgrad: [X, K] (X = R rows in group order, or T tokens when rows is set)
+  const void* x;  // fwd, wgrad: [R, K] in group order; [x_rows, K] tokens when rows is set
   int64_t ldx, x_rows;
-  const int* rows;  // [R] token of each row, or null
+  const int* rows;  // [R] token of each row, or null (set for few rows only)
   const void* w;    // fwd, dgrad: [G, K, N]
   const void* dy;   // dgrad, wgrad: [R, N]
   int64_t lddy;
@@ -93,11 +93,15 @@ struct GroupedArgs {
   void* out;  // fwd [R, N], dgrad [R, K], wgrad [G, K, N]
   int out_dtype;  // fwd: dtype; dgrad: dtype or fp32; wgrad: any
   int accumulate;  // wgrad: fp32 out += result
+  float* work;     // wgrad: grouped_work_floats() floats of scratch
   int* status;
   uint64_t timeout_ns;
 };
 
 void grouped_gemm(const GroupedArgs& a, cudaStream_t s);
+int64_t grouped_work_floats(int G, int64_t R, int K, int N);
+// Forward products of this many rows stream the weights with plain loads, and gather x themselves.
+bool grouped_few_rows(int64_t rows);
 
 struct GroupSumArgs {  // out[g, n] = sum over the group's rows of y[r, n]
   const void* y;
@@ -108,7 +112,9 @@ struct GroupSumArgs {  // out[g, n] = sum over the group's rows of y[r, n]
   void* out;
   int out_dtype;
   int accumulate;
+  float* work;  // group_sum_work_floats() floats of scratch
 };
+int64_t group_sum_work_floats(int G, int64_t R, int N);
 void group_colsum(const GroupSumArgs& a, cudaStream_t s);
 
 }  // namespace flare

@@ -228,7 +228,12 @@ void fill(flare::GroupedArgs& a, const Tensor& offsets, const Tensor& like, int6
   a.timeout_ns = static_cast<uint64_t>(timeout_ns);
 }
 
-// y [R, N]: rows of x (or x[rows]) times their group's weight [G, K, N], plus its bias
+// The tokens' rows in group order (rows behind the last group: zeros)
+Tensor gather_rows(const Tensor& x, const Tensor& offsets, const Tensor& row_of) {
+  return std::get<0>(combine_backward(std::nullopt, row_of, std::nullopt, offsets, x, row_of.numel(), x.size(0), row_of.size(-1)));
+}
+
+// y [R, N]: rows of x (or, for few of them, x[rows]) times their group's weight [G, K, N], plus its bias
 Tensor grouped_forward(const Tensor& x, const Tensor& w, const optional<Tensor>& bias, const Tensor& offsets, const optional<Tensor>& rows,
                        int64_t status, int64_t timeout_ns) {
   check_rows(x, "grouped_linear");
@@ -284,13 +289,17 @@ Tensor grouped_input_grad(const Tensor& dy, const Tensor& w, const Tensor& offse
   return dx;
 }
 
-// dW [G, K, N] and db [G, N], where they are given: written, or (fp32 only) added to
-void grouped_weight_grad(const Tensor& x, const Tensor& dy, const Tensor& offsets, const optional<Tensor>& rows, const optional<Tensor>& dw,
-                         bool accumulate, const optional<Tensor>& db, bool accumulate_bias, int64_t G, int64_t status, int64_t timeout_ns) {
+// dW [G, K, N], written or (fp32 only) added to.  x is in group order.
+void grouped_weight_grad(const Tensor& x, const Tensor& dy, const Tensor& offsets, const Tensor& dw, bool accumulate, int64_t G,
+                         int64_t status, int64_t timeout_ns) {
   check_rows(x, "grouped_linear");
   check_rows(dy, "grouped_linear gradient");
   const c10::cuda::CUDAGuard guard(x.device());
-  TORCH_CHECK(x.scalar_type() == dy.scalar_type() && x.device() == dy.device(), "grouped_linear: type of the gradient");
+  TORCH_CHECK(x.scalar_type() == dy.scalar_type() && x.device() == dy.device() && x.size(0) == dy.size(0),
+              "grouped_linear: gradient of another type or size");
+  TORCH_CHECK(dw.is_contiguous() && dw.device() == x.device() && dw.numel() == G * x.size(1) * dy.size(1) &&
+                  (!accumulate || dw.scalar_type() == at::kFloat),
+              "grouped_linear: weight gradient [groups, in, out], accumulated in float32");
   flare::GroupedArgs a{};
   a.mode = flare::kGroupedWgrad;
   a.dtype = code_of(x.scalar_type());
@@ -300,40 +309,42 @@ void grouped_weight_grad(const Tensor& x, const Tensor& dy, const Tensor& offset
   a.dy = dy.data_ptr();
   a.lddy = pitch(dy);
   a.R = dy.size(0);
-  if (rows.has_value()) a.rows = ints(*rows, x, a.R, "rows");
-  else TORCH_CHECK(x.size(0) == a.R, "grouped_linear: gradient of another size");
   a.K = static_cast<int>(x.size(1));
   a.N = static_cast<int>(dy.size(1));
   fill(a, offsets, x, G, status, timeout_ns);
-  const bool none = a.x_rows == 0 || a.R == 0;
-  if (dw.has_value()) {
-    TORCH_CHECK(dw->is_contiguous() && dw->device() == x.device() && dw->numel() == G * x.size(1) * dy.size(1) &&
-                    (!accumulate || dw->scalar_type() == at::kFloat),
-                "grouped_linear: weight gradient [groups, in, out], accumulated in float32");
-    if (none && !accumulate) dw->zero_();
-    a.out = dw->data_ptr();
-    a.out_dtype = code_of(dw->scalar_type());
-    a.accumulate = accumulate ? 1 : 0;
-    if (!none) flare::grouped_gemm(a, stream());
+  a.out = dw.data_ptr();
+  a.out_dtype = code_of(dw.scalar_type());
+  a.accumulate = accumulate ? 1 : 0;
+  const int64_t scratch = flare::grouped_work_floats(a.G, a.R, a.K, a.N);
+  Tensor work;
+  if (scratch > 0) {
+    work = empty({scratch}, x, at::kFloat);
+    a.work = work.data_ptr<float>();
   }
-  if (db.has_value()) {
-    TORCH_CHECK(db->is_contiguous() && db->device() == x.device() && db->numel() == G * dy.size(1) &&
-                    (!accumulate_bias || db->scalar_type() == at::kFloat),
-                "grouped_linear: bias gradient [groups, out], accumulated in float32");
-    if (none && !accumulate_bias) db->zero_();
-    flare::GroupSumArgs b{};
-    b.y = a.dy;
-    b.ldy = a.lddy;
-    b.R = a.R;
-    b.dtype = a.dtype;
-    b.offsets = a.offsets;
-    b.G = a.G;
-    b.N = a.N;
-    b.out = db->data_ptr();
-    b.out_dtype = code_of(db->scalar_type());
-    b.accumulate = accumulate_bias ? 1 : 0;
-    if (!none) flare::group_colsum(b, stream());
-  }
+  if (a.R > 0) flare::grouped_gemm(a, stream());
+  else if (!accumulate) dw.zero_();
+}
+
+// db [G, N], written or (fp32 only) added to
+void group_sums(const Tensor& dy, const Tensor& offsets, const Tensor& db, bool accumulate, int64_t G) {
+  const c10::cuda::CUDAGuard guard(dy.device());
+  TORCH_CHECK(db.is_contiguous() && db.device() == dy.device() && db.numel() == G * dy.size(1) && (!accumulate || db.scalar_type() == at::kFloat),
+              "grouped_linear: bias gradient [groups, out], accumulated in float32");
+  flare::GroupSumArgs b{};
+  b.y = dy.data_ptr();
+  b.ldy = pitch(dy);
+  b.R = dy.size(0);
+  b.dtype = code_of(dy.scalar_type());
+  b.offsets = ints(offsets, dy, G + 1, "offsets");
+  b.G = static_cast<int>(G);
+  b.N = static_cast<int>(dy.size(1));
+  b.out = db.data_ptr();
+  b.out_dtype = code_of(db.scalar_type());
+  b.accumulate = accumulate ? 1 : 0;
+  const Tensor work = empty({flare::group_sum_work_floats(b.G, b.R, b.N)}, dy, at::kFloat);
+  b.work = work.data_ptr<float>();
+  if (b.R > 0) flare::group_colsum(b, stream());
+  else if (!accumulate) db.zero_();
 }
 
 // ------------------------------------------------------------ graph nodes
@@ -358,6 +369,7 @@ Tensor tma_rows(const Tensor& t) {
 
 struct RouteFn : torch::autograd::Function<RouteFn> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, int64_t k) {
+    ctx->set_materialize_grads(false);
     auto [experts, weights, offsets, rows, row_of] = route_topk(logits, k);
     ctx->save_for_backward({experts, weights});
     ctx->saved_data["n"] = logits.size(2);
@@ -415,51 +427,63 @@ struct CombineFn : torch::autograd::Function<CombineFn> {
 // buffer) gets its gradient added there by the kernel; others get a gradient of their own type.
 struct GroupedLinearFn : torch::autograd::Function<GroupedLinearFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const optional<Tensor>& bias, const Tensor& offsets,
-                        const optional<Tensor>& rows, const optional<Tensor>& row_of, const optional<Tensor>& flat_w,
-                        const optional<Tensor>& flat_b, const Tensor& w, int64_t status, int64_t timeout_ns) {
-    Tensor y = grouped_forward(x, w, bias, offsets, rows, status, timeout_ns);
-    ctx->save_for_backward({x, w, offsets, rows.value_or(Tensor()), row_of.value_or(Tensor())});
-    ctx->saved_data["flat_w"] = flat_w;
-    ctx->saved_data["flat_b"] = flat_b;
-    ctx->saved_data["wshape"] = weight.sizes();
-    ctx->saved_data["wtype"] = static_cast<int64_t>(weight.scalar_type());
+                        const optional<Tensor>& row_of, const optional<Tensor>& flat_w, const optional<Tensor>& flat_b, const Tensor& w,
+                        int64_t status, int64_t timeout_ns) {
+    // The gathered rows are kept for the weight gradient: they are a small part of what a block keeps
+    // (in against 2h + h values a row), and gathering them again costs as much as the first time.
+    const Tensor xr = row_of.has_value() ? gather_rows(x, offsets, *row_of) : x;
+    Tensor y = grouped_forward(xr, w, bias, offsets, std::nullopt, status, timeout_ns);
+    auto& d = ctx->saved_data;
+    d["x?"] = x.requires_grad();
+    d["w?"] = weight.requires_grad();
+    d["b?"] = bias.has_value() && bias->requires_grad();
+    ctx->save_for_backward({weight.requires_grad() ? xr : Tensor(), x.requires_grad() ? w : Tensor(), offsets, row_of.value_or(Tensor())});
+    d["tokens"] = x.size(0);
+    d["flat_w"] = flat_w;
+    d["flat_b"] = flat_b;
+    d["groups"] = w.sizes();
+    d["wshape"] = weight.sizes();
+    d["wtype"] = static_cast<int64_t>(weight.scalar_type());
     if (bias.has_value()) {
-      ctx->saved_data["bshape"] = bias->sizes();
-      ctx->saved_data["btype"] = static_cast<int64_t>(bias->scalar_type());
+      d["bshape"] = bias->sizes();
+      d["btype"] = static_cast<int64_t>(bias->scalar_type());
     }
-    ctx->saved_data["x?"] = x.requires_grad();
-    ctx->saved_data["w?"] = weight.requires_grad();
-    ctx->saved_data["b?"] = bias.has_value() && bias->requires_grad();
-    ctx->saved_data["status"] = status;
-    ctx->saved_data["timeout"] = timeout_ns;
+    d["status"] = status;
+    d["timeout"] = timeout_ns;
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     once("grouped_linear");
-    variable_list out(11);
+    variable_list out(10);
     if (!g[0].defined()) return out;
     const auto saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &w = saved[1], &offsets = saved[2], &rows = saved[3], &row_of = saved[4];
+    const Tensor &x = saved[0], &w = saved[1], &offsets = saved[2], &row_of = saved[3];
     auto& d = ctx->saved_data;
     const int64_t status = d["status"].toInt(), timeout = d["timeout"].toInt();
     const Tensor dy = tma_rows(g[0]);
     if (d["x?"].toBool() && ctx->needs_input_grad(0)) {
-      if (rows.defined()) {  // a token's gradient is the sum over its rows: kept in fp32 until it is complete
+      if (row_of.defined()) {  // a token's gradient is the sum over its rows: kept in fp32 until it is complete
         const Tensor dr = grouped_input_grad(dy, w, offsets, at::kFloat, status, timeout);
-        out[0] = combine_forward(dr, row_of, std::nullopt, x.size(0), row_of.size(-1), x.scalar_type());
+        out[0] = combine_forward(dr, row_of, std::nullopt, d["tokens"].toInt(), row_of.size(-1), dy.scalar_type());
       } else {
-        out[0] = grouped_input_grad(dy, w, offsets, x.scalar_type(), status, timeout);
+        out[0] = grouped_input_grad(dy, w, offsets, dy.scalar_type(), status, timeout);
       }
     }
     const bool need_w = d["w?"].toBool() && ctx->needs_input_grad(1), need_b = d["b?"].toBool() && ctx->needs_input_grad(2);
     if (!need_w && !need_b) return out;
+    const auto groups = d["groups"].toIntVector();
     const optional<Tensor> flat_w = d["flat_w"].toOptional<Tensor>(), flat_b = d["flat_b"].toOptional<Tensor>();
     Tensor dw, db;
-    if (need_w) dw = flat_w.has_value() ? flat_w->view(w.sizes()) : empty(w.sizes(), w, static_cast<at::ScalarType>(d["wtype"].toInt()));
-    if (need_b) db = flat_b.has_value() ? flat_b->view({-1}) : empty(d["bshape"].toIntVector(), w, static_cast<at::ScalarType>(d["btype"].toInt()));
-    grouped_weight_grad(x, dy, offsets, some(rows), some(dw), flat_w.has_value(), some(db), flat_b.has_value(), w.size(0), status, timeout);
-    if (need_w && !flat_w.has_value()) out[1] = dw.view(d["wshape"].toIntVector());
-    if (need_b && !flat_b.has_value()) out[2] = db;
+    if (need_w) {
+      dw = flat_w.has_value() ? flat_w->view(groups) : empty(groups, dy, static_cast<at::ScalarType>(d["wtype"].toInt()));
+      grouped_weight_grad(x, dy, offsets, dw, flat_w.has_value(), groups[0], status, timeout);
+      if (!flat_w.has_value()) out[1] = dw.view(d["wshape"].toIntVector());
+    }
+    if (need_b) {
+      db = flat_b.has_value() ? flat_b->view({-1}) : empty(d["bshape"].toIntVector(), dy, static_cast<at::ScalarType>(d["btype"].toInt()));
+      group_sums(dy, offsets, db, flat_b.has_value(), groups[0]);
+      if (!flat_b.has_value()) out[2] = db;
+    }
     return out;
   }
 };
@@ -498,7 +522,9 @@ Tensor grouped_linear_op(const Tensor& x, const Tensor& weight, const optional<T
   Tensor w = weight.detach().reshape({-1, weight.size(-2), weight.size(-1)}).to(x.scalar_type()).contiguous();
   if (reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 != 0) w = w.clone();
   if (wants({&v, &weight}) || (b.has_value() && wants({&*b})))
-    return GroupedLinearFn::apply(v, weight, b, offsets, rows, row_of, flat_w, flat_b, w, status, timeout_ns);
+    return GroupedLinearFn::apply(v, weight, b, offsets, row_of, flat_w, flat_b, w, status, timeout_ns);
+  if (rows.has_value() && !flare::grouped_few_rows(rows->numel()))
+    return grouped_forward(gather_rows(v, offsets, *row_of), w, b, offsets, std::nullopt, status, timeout_ns);
   return grouped_forward(v, w, b, offsets, rows, status, timeout_ns);
 }
 

@@ -13,11 +13,14 @@
 // A persistent grid walks output tiles (n fastest: the tiles in flight share a
 // group's weights in L2 and the rows of a few tiles).  Per CTA: warp 0 loads
 // (TMA, a STAGES-deep ring of 128-byte-swizzled tiles), warp 1 issues the MMAs
-// into one of two TMEM accumulators, warps 2..5 drain the other: the epilogue of
-// a tile overlaps the mainloop of the next.  Rows gathered by index, and rows of
-// the weight gradient's last, partial step, are fetched four at a time by index
-// (a row outside the tensor reads as zeros: the next group's rows, and whatever
-// infinities are in them, never enter a product).
+// into one of two TMEM accumulators, warps 2..9 drain the other: the epilogue of
+// a tile overlaps the mainloop of the next (with K = 512 a mainloop is 4096 cycles,
+// and four warps took longer than that to write 256 x 256 values).  The rows of the weight gradient's
+// last, partial step are fetched four at a time by index (a row outside the tensor
+// reads as zeros: the next group's rows, and whatever infinities are in them, never
+// enter a product).  Rows are gathered from the tokens by a kernel of their own
+// before the product: fetched by index inside it, four rows cost 45 ns of a CTA's
+// load unit, 1293 us against 432 us for 131072 x 512 x 4096.
 // Variants: CTA pairs on 256 x 256 tiles (each CTA stages half of B, which halves
 // its operand traffic), one CTA on 128 x 128 or 128 x 64 tiles.
 // Every sum is held in fp32 and rounded once.  Every wait is bounded.
@@ -38,20 +41,18 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn();  // gemm_tcgen05.cu
 namespace {
 
 constexpr int kBK = 64;          // contraction step: one 128-byte swizzle atom of 16-bit values
-constexpr int kThreads = 192;    // producer, MMA issuer, four epilogue warps
-constexpr int kEpiWarps = 4;
+constexpr int kEpiWarps = 8;     // two for each quarter of the TMEM lanes, half of the columns each
+constexpr int kThreads = 64 + 32 * kEpiWarps;  // and the producer and MMA issuer warps
 constexpr int kTileA = 128 * kBK * 2;
 
 struct GP {
   const int* offsets;
   int G, R;
-  const int* rows;
-  int x_rows;    // rows of x (an index of this value reads zeros)
-  int dy_rows;
   int Mo;        // weight gradient: output rows of a group
   int No;        // output columns
   int Kc;        // forward, input gradient: contraction length
   int mt, nt;    // tiles of a group's output rows (weight gradient) and columns
+  int slices;    // weight gradient: parts of a group's rows, each with an output of its own
   void* out;
   int64_t ldo;
   int out_dtype, accumulate;
@@ -68,9 +69,9 @@ struct Smem {
   static constexpr int kTileB = kBNh * kBK * 2;
   static constexpr int kStage = kTileA + kTileB;
   static constexpr int kOffB = STAGES * kTileA;
-  static constexpr int kOffEpi = kOffB + STAGES * kTileB;       // 4 KiB per epilogue warp
-  static constexpr int kOffBias = kOffEpi + kEpiWarps * 4096;   // 64 floats per epilogue warp
-  static constexpr int kOffPre = kOffBias + kEpiWarps * 256;    // tile prefix of the groups
+  static constexpr int kOffEpi = kOffB + STAGES * kTileB;       // 2 KiB per epilogue warp
+  static constexpr int kOffBias = kOffEpi + kEpiWarps * 2048;   // 32 floats per epilogue warp
+  static constexpr int kOffPre = kOffBias + kEpiWarps * 128;    // tile prefix of the groups, or their order
   static constexpr int kOffBar = kOffPre + (kGroupedMaxGroups + 2) * 4;
   static constexpr int kBytes = kOffBar + (2 * STAGES + 4) * 8 + 16;
   static constexpr int kAlloc = kBytes + 1024;
@@ -84,41 +85,57 @@ __device__ __forceinline__ int2 group_range(const GP& p, int g) {
 }
 
 struct Tile {
-  int g, m0, n0, lo, hi, steps;
+  int g, m0, n0;
+  int lo, hi;    // rows: of the group, or of the weight gradient's slice
+  int steps, slice;
 };
 
-// Walks this CTA's (or pair's) tiles in order.
+constexpr int kSortGroups = 512;
+
+// Walks this CTA's (or pair's) tiles in order.  The weight gradient's tiles differ in length: they
+// come by falling size of their group, dealt out back and forth, so that every CTA gets about the
+// same number of steps.
 template <int MODE, int BM, int BN>
 struct Walk {
   const GP& p;
   const int* pre;
-  int u, step, total, g;
+  int turn, me, step, total, g;
   __device__ Walk(const GP& p_, const int* pre_, int first, int step_)
-      : p(p_), pre(pre_), u(first), step(step_), total(MODE == kGroupedWgrad ? p_.G * p_.mt * p_.nt : pre_[p_.G] * p_.nt), g(0) {}
+      : p(p_), pre(pre_), turn(0), me(first), step(step_),
+        total(MODE == kGroupedWgrad ? p_.G * p_.mt * p_.nt * p_.slices : pre_[p_.G] * p_.nt), g(0) {}
   __device__ bool next(Tile& t) {
-    if (u >= total) return false;
+    int u = turn * step + me;
+    if (MODE == kGroupedWgrad && (turn & 1)) u = turn * step + (step - 1 - me);
+    if (u >= total) return false;  // so is every later one
+    ++turn;
     const int n = u % p.nt;
     int m = u / p.nt;
+    t.n0 = n * BN;
+    t.slice = 0;
     if constexpr (MODE == kGroupedWgrad) {
-      g = m / p.mt;
-      m -= g * p.mt;
+      const int per = p.mt * p.slices, at = m / per;
+      m -= at * per;
+      t.slice = m / p.mt;
+      m -= t.slice * p.mt;
+      t.g = p.G <= kSortGroups ? pre[at] : at;
+      const int2 r = group_range(p, t.g);
+      t.m0 = m * BM;
+      const int steps = (r.y - r.x + kBK - 1) / kBK;
+      const int s0 = static_cast<int>(static_cast<int64_t>(steps) * t.slice / p.slices);
+      const int s1 = static_cast<int>(static_cast<int64_t>(steps) * (t.slice + 1) / p.slices);
+      t.lo = r.x + s0 * kBK;
+      t.hi = min(r.y, r.x + s1 * kBK);
+      t.steps = s1 - s0;
     } else {
       while (pre[g + 1] <= m) ++g;
       m -= pre[g];
-    }
-    const int2 r = group_range(p, g);
-    t.g = g;
-    t.lo = r.x;
-    t.hi = r.y;
-    t.n0 = n * BN;
-    if constexpr (MODE == kGroupedWgrad) {
-      t.m0 = m * BM;
-      t.steps = (r.y - r.x + kBK - 1) / kBK;
-    } else {
+      const int2 r = group_range(p, g);
+      t.g = g;
+      t.lo = r.x;
+      t.hi = r.y;
       t.m0 = r.x + m * BM;
       t.steps = (p.Kc + kBK - 1) / kBK;
     }
-    u += step;
     return true;
   }
 };
@@ -138,27 +155,27 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, bool bf16) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// 64 columns of 32 rows (lane = row) to out, through 4 KiB of shared memory: eight lanes write one
-// row's 128 bytes (64 values of 16 bits, or 32 of fp32 at a time) instead of every lane 16 bytes of
-// its own row.  16-byte pieces lie at piece ^ (row % 8): no bank is hit twice on either side.
-__device__ __forceinline__ void store_chunk(const GP& p, float (&v)[64], int64_t row0, int rows, int col, int64_t base,
+// 32 columns of 32 rows (lane = row) to out, through 2 KiB of shared memory: four lanes write 64
+// bytes of one row (32 values of 16 bits, or 16 of fp32 at a time) instead of every lane 16 bytes
+// of its own row.  16-byte pieces lie at piece ^ (row / 2 % 4): no bank is hit twice on either side.
+__device__ __forceinline__ void store_chunk(const GP& p, const float (&v)[32], int64_t row0, int rows, int col, int64_t base,
                                             uint8_t* stage) {
-  const int lane = lane_id(), q = lane & 7;
+  const int lane = lane_id(), q = lane & 3, key = (lane >> 1) & 3;
   if (p.out_dtype == kF32) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        const int j = h * 32 + c * 4;
-        *reinterpret_cast<float4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+      for (int c = 0; c < 4; ++c) {
+        const int j = h * 16 + c * 4;
+        *reinterpret_cast<float4*>(stage + lane * 64 + ((c ^ key) << 4)) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
       }
       __syncwarp();
-      float* o = static_cast<float*>(p.out) + base + row0 * p.ldo + col + h * 32 + q * 4;
+      float* o = static_cast<float*>(p.out) + base + row0 * p.ldo + col + h * 16 + q * 4;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = i * 4 + (lane >> 3);
-        float4 u = *reinterpret_cast<const float4*>(stage + r * 128 + ((q ^ (r & 7)) << 4));
-        if (r < rows && col + h * 32 + q * 4 < p.No) {
+      for (int i = 0; i < 4; ++i) {
+        const int r = i * 8 + (lane >> 2);
+        float4 u = *reinterpret_cast<const float4*>(stage + r * 64 + ((q ^ ((r >> 1) & 3)) << 4));
+        if (r < rows && col + h * 16 + q * 4 < p.No) {
           if (p.accumulate) u = f4_add(u, *reinterpret_cast<const float4*>(o + r * p.ldo));
           *reinterpret_cast<float4*>(o + r * p.ldo) = u;
         }
@@ -169,23 +186,29 @@ __device__ __forceinline__ void store_chunk(const GP& p, float (&v)[64], int64_t
   }
   const bool bf = p.out_dtype == kBF16;
 #pragma unroll
-  for (int c = 0; c < 8; ++c) {
+  for (int c = 0; c < 4; ++c) {
     uint4 u;
     u.x = pack2(v[8 * c], v[8 * c + 1], bf);
     u.y = pack2(v[8 * c + 2], v[8 * c + 3], bf);
     u.z = pack2(v[8 * c + 4], v[8 * c + 5], bf);
     u.w = pack2(v[8 * c + 6], v[8 * c + 7], bf);
-    *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = u;
+    *reinterpret_cast<uint4*>(stage + lane * 64 + ((c ^ key) << 4)) = u;
   }
   __syncwarp();
   uint16_t* o = static_cast<uint16_t*>(p.out) + base + row0 * p.ldo + col + q * 8;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = i * 4 + (lane >> 3);
-    const uint4 u = *reinterpret_cast<const uint4*>(stage + r * 128 + ((q ^ (r & 7)) << 4));
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * 8 + (lane >> 2);
+    const uint4 u = *reinterpret_cast<const uint4*>(stage + r * 64 + ((q ^ ((r >> 1) & 3)) << 4));
     if (r < rows && col + q * 8 < p.No) *reinterpret_cast<uint4*>(o + r * p.ldo) = u;
   }
   __syncwarp();
+}
+
+// Keeps uses of a TMEM load's registers behind the wait for it.
+__device__ __forceinline__ void regs_ready(uint32_t (&r)[32]) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j) asm volatile("" : "+r"(r[j]));
 }
 
 // Rows outside every group (before the first, behind the last) become zeros.
@@ -201,8 +224,8 @@ __device__ __forceinline__ void zero_outside(const GP& p, int warp, int warps) {
   }
 }
 
-// ta / tb: tiles of A and B; ga / gb: the same tensors with boxes of one row (gathered rows).
-template <int MODE, bool PAIR, int BN, int STAGES, bool GATHER>
+// ta / tb: tiles of A and B; ga / gb: the same tensors with boxes of one row (rows by index).
+template <int MODE, bool PAIR, int BN, int STAGES>
 __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& ga,
                                              const CUtensorMap& gb, const GP& p) {
   using L = Smem<PAIR, BN, STAGES>;
@@ -264,6 +287,22 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
       }
     }
   }
+  if constexpr (MODE == kGroupedWgrad) {
+    if (p.G <= kSortGroups) {  // by falling size, equal ones in order
+      int* size = pre + kSortGroups;
+      for (int g = threadIdx.x; g < p.G; g += kThreads) {
+        const int2 r = group_range(p, g);
+        size[g] = r.y - r.x;
+      }
+      __syncthreads();
+      for (int g = threadIdx.x; g < p.G; g += kThreads) {
+        const int mine = size[g];
+        int at = 0;
+        for (int o = 0; o < p.G; ++o) at += size[o] > mine || (size[o] == mine && o < g);
+        pre[at] = g;
+      }
+    }
+  }
   if (blockIdx.x == 0) {  // a group that ends before it starts, or outside the rows, is reported
     for (int g = threadIdx.x; g < p.G; g += kThreads)
       if (p.offsets[g] < 0 || p.offsets[g + 1] < p.offsets[g] || p.offsets[g + 1] > p.R)
@@ -293,24 +332,13 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
       if constexpr (PAIR) sm100::tma_gather4_pair(dst, &m, sm100::mapa_shared(&full[s], 0), x, r);
       else sm100::tma_gather4(dst, &m, &full[s], x, r);
     };
-    // rows r .. r + 3 of x: their tokens, or the rows themselves; outside [.., hi): a row of zeros
-    auto row4 = [&](int r, int hi, const int* rows, int none) {
-      int v[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int x = r + i < hi ? (rows != nullptr ? rows[r + i] : r + i) : none;
-        v[i] = static_cast<unsigned>(x) < static_cast<unsigned>(none) ? x : none;
-      }
-      return make_int4(v[0], v[1], v[2], v[3]);
+    // rows r .. r + 3, a row of zeros in the place of those from hi on
+    auto row4 = [&](int r, int hi) {
+      return make_int4(r < hi ? r : p.R, r + 1 < hi ? r + 1 : p.R, r + 2 < hi ? r + 2 : p.R, r + 3 < hi ? r + 3 : p.R);
     };
     while (ok && walk.next(t)) {
-      int4 ar = make_int4(0, 0, 0, 0);
-      if constexpr (MODE == kGroupedFwd && GATHER) ar = row4(t.m0 + rank * 128 + 4 * lane, t.hi, p.rows, p.x_rows);
       for (int k = 0; k < t.steps; ++k, ++it) {
         const int s = it % STAGES;
-        int4 xr = make_int4(0, 0, 0, 0);
-        const int r0 = t.lo + k * kBK;
-        if constexpr (MODE == kGroupedWgrad && GATHER) xr = row4(r0 + 4 * (lane & 15), t.hi, p.rows, p.x_rows);
         if (it >= STAGES && !sm100::mbar_wait(&empty[s], ((it / STAGES) - 1) & 1, p.timeout_ns, p.status, 400 + s)) ok = false;
         if (!__all_sync(0xffffffffu, ok)) {
           ok = false;
@@ -321,9 +349,8 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
         if (lane == 0 && rank == 0) sm100::mbar_arrive_expect_tx(&full[s], (PAIR ? 2 : 1) * L::kStage);
         if constexpr (MODE != kGroupedWgrad) {
           const int k0 = k * kBK;
-          if constexpr (GATHER) gather(sa + lane * 512, ga, s, k0, ar);
           if (lane == 0) {
-            if constexpr (!GATHER) load2(sa, ta, s, k0, t.m0 + rank * 128);
+            load2(sa, ta, s, k0, t.m0 + rank * 128);
             if constexpr (B_MN) {
 #pragma unroll
               for (int j = 0; j < L::kBNh / 64; ++j) load3(sb + j * 8192, tb, s, t.n0 + rank * L::kBNh + 64 * j, k0, t.g);
@@ -332,26 +359,21 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
             }
           }
         } else {
-          const int ma = t.m0 + rank * 128, nb = t.n0 + rank * L::kBNh, sub = lane & 15, half = lane >> 4;
-          const bool whole = r0 + kBK <= t.hi;
-          if constexpr (GATHER) {
-            gather(sa + half * 8192 + sub * 512, ga, s, ma + 64 * half, xr);
-          } else if (!whole) {
-            gather(sa + half * 8192 + sub * 512, ga, s, ma + 64 * half, row4(r0 + 4 * sub, t.hi, nullptr, p.x_rows));
-          }
-          if (!whole) {
-            const int4 br = row4(r0 + 4 * sub, t.hi, nullptr, p.dy_rows);
-#pragma unroll
-            for (int j = 0; j < L::kBNh / 64; j += 2)
-              if (j + half < L::kBNh / 64) gather(sb + (j + half) * 8192 + sub * 512, gb, s, nb + 64 * (j + half), br);
-          }
-          if (lane == 0 && whole) {
-            if constexpr (!GATHER) {
+          const int r0 = t.lo + k * kBK, ma = t.m0 + rank * 128, nb = t.n0 + rank * L::kBNh;
+          if (r0 + kBK <= t.hi) {
+            if (lane == 0) {
               load2(sa, ta, s, ma, r0);
               load2(sa + 8192, ta, s, ma + 64, r0);
-            }
 #pragma unroll
-            for (int j = 0; j < L::kBNh / 64; ++j) load2(sb + j * 8192, tb, s, nb + 64 * j, r0);
+              for (int j = 0; j < L::kBNh / 64; ++j) load2(sb + j * 8192, tb, s, nb + 64 * j, r0);
+            }
+          } else {
+            const int sub = lane & 15, half = lane >> 4;
+            const int4 r = row4(r0 + 4 * sub, t.hi);
+            gather(sa + half * 8192 + sub * 512, ga, s, ma + 64 * half, r);
+#pragma unroll
+            for (int j = 0; j < L::kBNh / 64; j += 2)
+              if (j + half < L::kBNh / 64) gather(sb + (j + half) * 8192 + sub * 512, gb, s, nb + 64 * (j + half), r);
           }
         }
       }
@@ -403,58 +425,53 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
   } else {
     // ------------------------------------------------------------ epilogue
     const int quarter = warp & 3;  // the TMEM lanes that this warp may read
-    uint8_t* stage = sm + L::kOffEpi + (warp - 2) * 4096;
-    float* bias = reinterpret_cast<float*>(sm + L::kOffBias + (warp - 2) * 256);
+    const int c0 = ((warp - 2) >> 2) * (BN / 2);
+    uint8_t* stage = sm + L::kOffEpi + (warp - 2) * 2048;
+    float* bias = reinterpret_cast<float*>(sm + L::kOffBias + (warp - 2) * 128);
     if constexpr (MODE != kGroupedWgrad) zero_outside(p, blockIdx.x * kEpiWarps + warp - 2, gridDim.x * kEpiWarps);
     uint32_t i = 0;
     while (walk.next(t)) {
       const int buf = i & 1;
       const bool any = t.steps > 0;
-      if (any) {
-        bool ok = sm100::mbar_wait(&acc_full[buf], (i >> 1) & 1, p.timeout_ns, p.status, 460 + buf);
-        if (!__all_sync(0xffffffffu, ok)) break;
-        sm100::tc_fence_after();
-      }
-      const int64_t row0 = t.m0 + rank * 128 + quarter * 32;
-      const int rows = min(32, (MODE == kGroupedWgrad ? p.Mo : t.hi) - static_cast<int>(row0));
-      const int64_t base = MODE == kGroupedWgrad ? static_cast<int64_t>(t.g) * p.Mo * p.ldo : 0;
-      for (int c = 0; c < BN; c += 64) {
-        const int col = t.n0 + c;
-        if (col >= p.No || rows <= 0) break;  // warp-uniform
-        float v[64];
-        if (any) {
-          uint32_t r[2][32];
-          const uint32_t at = tmem + buf * BN + c + (static_cast<uint32_t>(quarter * 32) << 16);
-          sm100::tmem_ld_32x32b_x32(at, r[0]);
-          sm100::tmem_ld_32x32b_x32(at + 32, r[1]);
-          if (MODE == kGroupedFwd && p.bias != nullptr) {
+      const int row0 = t.m0 + rank * 128 + quarter * 32;
+      const int rows = min(32, (MODE == kGroupedWgrad ? p.Mo : t.hi) - row0);
+      const int chunks = rows > 0 ? min(BN / 64, (p.No - t.n0 - c0 + 31) / 32) : 0;  // of 32 columns, with some inside
+      const int64_t base = MODE == kGroupedWgrad ? (static_cast<int64_t>(t.slice) * p.G + t.g) * p.Mo * p.ldo : 0;
+      auto finish = [&](uint32_t (&r)[32], int c) {
+        const int col = t.n0 + c0 + c * 32;
+        float v[32];
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-              bias[h * 32 + lane] = col + h * 32 + lane < p.No ? load_any(p.bias, static_cast<int64_t>(t.g) * p.No + col + h * 32 + lane, p.bias_dtype) : 0.f;
-            __syncwarp();
+        for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+        if (MODE == kGroupedFwd && p.bias != nullptr) {
+          bias[lane] = col + lane < p.No ? load_any(p.bias, static_cast<int64_t>(t.g) * p.No + col + lane, p.bias_dtype) : 0.f;
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const float4 b = *reinterpret_cast<const float4*>(bias + j);
+            v[j] += b.x, v[j + 1] += b.y, v[j + 2] += b.z, v[j + 3] += b.w;
           }
-          sm100::tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 64; ++j) {
-            asm volatile("" : "+r"(r[j >> 5][j & 31]));
-            v[j] = __uint_as_float(r[j >> 5][j & 31]);
-          }
-          if (MODE == kGroupedFwd && p.bias != nullptr) {
-#pragma unroll
-            for (int j = 0; j < 64; j += 4) {
-              const float4 b = *reinterpret_cast<const float4*>(bias + j);
-              v[j] += b.x, v[j + 1] += b.y, v[j + 2] += b.z, v[j + 3] += b.w;
-            }
-            __syncwarp();
-          }
-        } else {
-          if (p.accumulate) break;
-#pragma unroll
-          for (int j = 0; j < 64; ++j) v[j] = 0.f;
         }
         store_chunk(p, v, row0, rows, col, base, stage);
-      }
+      };
       if (any) {
+        const bool ok = sm100::mbar_wait(&acc_full[buf], (i >> 1) & 1, p.timeout_ns, p.status, 460 + buf);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        sm100::tc_fence_after();
+        const uint32_t at = tmem + buf * BN + c0 + (static_cast<uint32_t>(quarter * 32) << 16);
+        uint32_t ra[32], rb[32];  // the next chunk is on its way while one is written
+        if (chunks > 0) sm100::tmem_ld_32x32b_x32(at, ra);
+        for (int c = 0; c < chunks; c += 2) {
+          sm100::tmem_ld_wait();
+          regs_ready(ra);
+          if (c + 1 < chunks) sm100::tmem_ld_32x32b_x32(at + (c + 1) * 32, rb);
+          finish(ra, c);
+          if (c + 1 < chunks) {
+            sm100::tmem_ld_wait();
+            regs_ready(rb);
+            if (c + 2 < chunks) sm100::tmem_ld_32x32b_x32(at + (c + 2) * 32, ra);
+            finish(rb, c + 1);
+          }
+        }
         sm100::tc_fence_before();
         __syncwarp();
         if (lane == 0) {
@@ -462,6 +479,11 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
           else sm100::mbar_arrive(&acc_empty[buf]);
         }
         ++i;
+      } else if (!p.accumulate) {  // a group without rows has a gradient of zeros
+        uint32_t zero[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) zero[j] = 0u;
+        for (int c = 0; c < chunks; ++c) finish(zero, c);
       }
     }
   }
@@ -474,18 +496,18 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
   }
 }
 
-template <int MODE, int BN, int STAGES, bool GATHER>
+template <int MODE, int BN, int STAGES>
 __global__ void __launch_bounds__(kThreads, 1)
     grouped_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
                    const __grid_constant__ CUtensorMap ga, const __grid_constant__ CUtensorMap gb, const __grid_constant__ GP p) {
-  grouped_body<MODE, false, BN, STAGES, GATHER>(ta, tb, ga, gb, p);
+  grouped_body<MODE, false, BN, STAGES>(ta, tb, ga, gb, p);
 }
-template <int MODE, int BN, int STAGES, bool GATHER>
+template <int MODE, int BN, int STAGES>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     grouped_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
                         const __grid_constant__ CUtensorMap ga, const __grid_constant__ CUtensorMap gb,
                         const __grid_constant__ GP p) {
-  grouped_body<MODE, true, BN, STAGES, GATHER>(ta, tb, ga, gb, p);
+  grouped_body<MODE, true, BN, STAGES>(ta, tb, ga, gb, p);
 }
 
 // ------------------------------------------------------------------- host
@@ -548,26 +570,24 @@ int resident(const void* kern, int smem, bool pair, int (&cache)[kMaxDevices]) {
   return cache[dev];
 }
 
-template <int MODE, bool PAIR, int BN, int STAGES, bool GATHER>
-void launch(const GroupedArgs& a, cudaStream_t s) {
+template <int MODE, bool PAIR, int BN, int STAGES>
+void launch(const GroupedArgs& a, cudaStream_t s, int slices = 1) {
   using L = Smem<PAIR, BN, STAGES>;
   constexpr int BM = PAIR ? 256 : 128;
   GP p{};
   p.offsets = a.offsets;
   p.G = a.G;
   p.R = static_cast<int>(a.R);
-  p.rows = a.rows;
-  p.x_rows = static_cast<int>(a.x_rows);
-  p.dy_rows = p.R;
   p.Mo = a.K;
   p.No = MODE == kGroupedDgrad ? a.K : a.N;
   p.Kc = MODE == kGroupedDgrad ? a.N : a.K;
   p.mt = ceil_div(a.K, BM);
   p.nt = ceil_div(p.No, BN);
-  p.out = a.out;
+  p.slices = slices;
+  p.out = slices > 1 ? a.work : a.out;
   p.ldo = p.No;
-  p.out_dtype = a.out_dtype;
-  p.accumulate = a.accumulate;
+  p.out_dtype = slices > 1 ? kF32 : a.out_dtype;
+  p.accumulate = slices > 1 ? 0 : a.accumulate;
   p.bias = MODE == kGroupedFwd ? a.bias : nullptr;
   p.bias_dtype = a.bias_dtype;
   p.idesc = sm100::make_idesc_16bit(BM, BN, MODE == kGroupedWgrad, MODE != kGroupedDgrad, a.dtype == kBF16);
@@ -575,31 +595,31 @@ void launch(const GroupedArgs& a, cudaStream_t s) {
   p.timeout_ns = a.timeout_ns;
   CUtensorMap ta, tb, ga, gb;
   if (MODE == kGroupedWgrad) {
-    ta = map2(a.x, a.dtype, a.K, a.x_rows, a.ldx, kBK);
-    ga = map2(a.x, a.dtype, a.K, a.x_rows, a.ldx, 1);
+    ta = map2(a.x, a.dtype, a.K, a.R, a.ldx, kBK);
+    ga = map2(a.x, a.dtype, a.K, a.R, a.ldx, 1);
     tb = map2(a.dy, a.dtype, a.N, a.R, a.lddy, kBK);
     gb = map2(a.dy, a.dtype, a.N, a.R, a.lddy, 1);
   } else {
     const int64_t wd[3] = {a.N, a.K, a.G}, wp[2] = {a.N, static_cast<int64_t>(a.K) * a.N};
     const int box_fwd[3] = {64, kBK, 1}, box_bwd[3] = {64, L::kBNh, 1};
     tb = make_map(a.w, a.dtype, 3, wd, wp, MODE == kGroupedFwd ? box_fwd : box_bwd);
-    if (MODE == kGroupedFwd) ta = map2(a.x, a.dtype, a.K, a.x_rows, a.ldx, GATHER ? 1 : 128);
+    if (MODE == kGroupedFwd) ta = map2(a.x, a.dtype, a.K, a.R, a.ldx, 128);
     else ta = map2(a.dy, a.dtype, a.N, a.R, a.lddy, 128);
     ga = ta;
     gb = tb;
   }
   // as many tiles as there can be: the groups' sizes are on the device
   const int64_t tiles = MODE == kGroupedWgrad
-                            ? static_cast<int64_t>(a.G) * p.mt * p.nt
+                            ? static_cast<int64_t>(a.G) * p.mt * p.nt * slices
                             : (a.R / BM + std::min<int64_t>(a.G, a.R)) * p.nt;
   FLARE_CHECK(tiles < (1ll << 31), "grouped products: too many tiles");
   static int cache[kMaxDevices];
   if constexpr (PAIR) {
-    auto kern = grouped_pair_kernel<MODE, BN, STAGES, GATHER>;
+    auto kern = grouped_pair_kernel<MODE, BN, STAGES>;
     const int n = static_cast<int>(std::min<int64_t>(std::max<int64_t>(1, tiles), resident(reinterpret_cast<const void*>(kern), L::kAlloc, true, cache)));
     kern<<<2 * n, kThreads, L::kAlloc, s>>>(ta, tb, ga, gb, p);
   } else {
-    auto kern = grouped_kernel<MODE, BN, STAGES, GATHER>;
+    auto kern = grouped_kernel<MODE, BN, STAGES>;
     const int n = static_cast<int>(std::min<int64_t>(std::max<int64_t>(1, tiles), resident(reinterpret_cast<const void*>(kern), L::kAlloc, false, cache)));
     kern<<<n, kThreads, L::kAlloc, s>>>(ta, tb, ga, gb, p);
   }
@@ -607,54 +627,301 @@ void launch(const GroupedArgs& a, cudaStream_t s) {
   count_launch();
 }
 
-template <int MODE, bool GATHER>
+// The slices of the weight gradient that its output tiles leave the machine idle without: a few
+// groups of a small weight and many rows.  Each is at least 512 rows of an average group.
+struct WgradShape {
+  bool pair;
+  int bn, slices;
+};
+WgradShape wgrad_shape(int G, int64_t R, int K, int N) {
+  WgradShape w;
+  w.pair = K > 128 && N > 128;
+  w.bn = w.pair ? 256 : N > 64 ? 128 : 64;
+  const int64_t tiles = static_cast<int64_t>(G) * ceil_div(K, w.pair ? 256 : 128) * ceil_div(N, w.bn);
+  const int64_t want = w.pair ? 148 : 296, most = std::min<int64_t>(64, R / G / 512);
+  w.slices = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, want / tiles)));
+  return w;
+}
+
+__global__ void __launch_bounds__(256) add_slices_kernel(const float* part, int64_t n, int slices, void* out, int dtype, int accumulate) {
+  for (int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4; i < n; i += static_cast<int64_t>(gridDim.x) * 1024) {
+    float4 v = *reinterpret_cast<const float4*>(part + i);
+#pragma unroll 4
+    for (int s = 1; s < slices; ++s) v = f4_add(v, *reinterpret_cast<const float4*>(part + s * n + i));
+    if (dtype == kF32) {
+      float4* o = reinterpret_cast<float4*>(static_cast<float*>(out) + i);
+      *o = accumulate ? f4_add(*o, v) : v;
+    } else {
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + i) = make_uint2(pack2(v.x, v.y, dtype == kBF16), pack2(v.z, v.w, dtype == kBF16));
+    }
+  }
+}
+
+template <int MODE>
 void pick(const GroupedArgs& a, cudaStream_t s) {
   const int no = MODE == kGroupedDgrad ? a.K : a.N;
   // rows of an average group fill a pair's 256 at least once, and both sides of the tile are used
-  const bool tall = MODE == kGroupedWgrad ? a.K > 128 : a.R >= 256ll * a.G;
-  if (tall && no > 128) launch<MODE, true, 256, 6, GATHER>(a, s);
-  else if (no > 64) launch<MODE, false, 128, 6, GATHER>(a, s);
-  else launch<MODE, false, 64, 8, GATHER>(a, s);
+  if (a.R >= 256ll * a.G && no > 128) launch<MODE, true, 256, 6>(a, s);
+  else if (no > 64) launch<MODE, false, 128, 6>(a, s);
+  else launch<MODE, false, 64, 8>(a, s);
+}
+
+void wgrad(const GroupedArgs& a, cudaStream_t s) {
+  const WgradShape w = wgrad_shape(a.G, a.R, a.K, a.N);
+  if (w.pair) launch<kGroupedWgrad, true, 256, 6>(a, s, w.slices);
+  else if (w.bn == 128) launch<kGroupedWgrad, false, 128, 6>(a, s, w.slices);
+  else launch<kGroupedWgrad, false, 64, 8>(a, s, w.slices);
+  if (w.slices > 1) {
+    const int64_t n = static_cast<int64_t>(a.G) * a.K * a.N;
+    add_slices_kernel<<<static_cast<int>(std::min<int64_t>((n + 1023) / 1024, 148 * 8)), 256, 0, s>>>(
+        static_cast<const float*>(a.work), n, w.slices, a.out, a.out_dtype, a.accumulate);
+    FLARE_CUDA_CHECK(cudaGetLastError());
+    count_launch();
+  }
+}
+
+// ------------------------------------------------------------- cluster sums
+// The CTAs of a cluster hold partial sums in shared memory; rank 0 adds them in order of rank.
+__device__ __forceinline__ float cluster_value(const float* local, uint32_t rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(sm100::mapa_shared(local, rank)) : "memory");
+  return v;
+}
+
+template <typename... Args>
+void launch_cluster(void (*kern)(Args...), dim3 grid, int threads, int cluster_z, cudaStream_t s, Args... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = cluster_z;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  FLARE_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, args...));
+  count_launch();
+}
+
+__device__ __forceinline__ void store_any(void* p, int64_t i, int dtype, float v) {
+  if (dtype == kF32) static_cast<float*>(p)[i] = v;
+  else if (dtype == kBF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  else static_cast<__half*>(p)[i] = __float2half_rn(v);
+}
+
+// ---------------------------------------------------------------- few rows
+// A serving step has a row or two in each chosen group: what counts is to stream those groups'
+// weights with every SM at work, and the tensor cores would multiply tiles of nothing.
+// Block = 64 columns of one chosen group (blockIdx.y-th of those that have rows), one slice of K
+// (a cluster's CTAs share the columns and K).  A thread owns 8 columns (one 16-byte load of a
+// weight row) of every 32nd row of the slice and up to MR rows of x; its partial sums meet by
+// shuffles, then through shared memory, then across the cluster, always in the same order.
+constexpr int kFewK = 512;  // a chunk of K whose x values are in shared memory
+constexpr int kFewRows = 4; // of a group at a time: 32 sums a thread, three blocks on an SM
+template <typename T, int MR>
+__device__ __forceinline__ void few_rows(const GroupedArgs& a, int g, int r0, int nr, int k0, int k1, float (*xs)[kFewRows],
+                                         float (*part)[kFewRows][64]) {
+  const int c8 = threadIdx.x & 7, kl = threadIdx.x >> 3, warp = warp_id(), lane = lane_id();
+  const int col = blockIdx.x * 64 + c8 * 8;
+  const bool in = col < a.N;
+  const T* w = static_cast<const T*>(a.w) + (static_cast<int64_t>(g) * a.K) * a.N + col;
+  float acc[MR][8];
+#pragma unroll
+  for (int m = 0; m < MR; ++m)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[m][i] = 0.f;
+  auto fetch = [&](uint4 (&u)[4], int kc, int kk, int kn) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      u[q] = in && kk + 32 * q < kn ? __ldg(reinterpret_cast<const uint4*>(w + static_cast<int64_t>(kc + kk + 32 * q) * a.N))
+                                    : make_uint4(0, 0, 0, 0);
+  };
+  for (int kc = k0; kc < k1; kc += kFewK) {
+    const int kn = min(kFewK, k1 - kc);
+    uint4 u[4];
+    fetch(u, kc, kl, kn);  // the first weights are on their way while x is fetched
+    __syncthreads();
+    const int m = threadIdx.x >> 6;  // a quarter of the block for each row
+    if (m < nr) {
+      const int row = a.rows != nullptr ? a.rows[r0 + m] : r0 + m;
+      const bool live = row >= 0 && row < a.x_rows;
+      const T* x = static_cast<const T*>(a.x) + row * a.ldx + kc;
+      for (int k = (threadIdx.x & 63); k < kn; k += 64) xs[k][m] = live ? to_f32(x[k]) : 0.f;
+    }
+    __syncthreads();
+    for (int kk = kl; kk < kn; kk += 128) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (kk + 32 * q < kn) {
+          const T* wv = reinterpret_cast<const T*>(&u[q]);
+          float x[MR];
+#pragma unroll
+          for (int j = 0; j < MR; ++j) x[j] = xs[kk + 32 * q][j];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float f = to_f32(wv[i]);
+#pragma unroll
+            for (int j = 0; j < MR; ++j) acc[j][i] = fmaf(x[j], f, acc[j][i]);
+          }
+        }
+      }
+      if (kk + 128 < kn) fetch(u, kc, kk + 128, kn);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < MR; ++j)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float v = acc[j][i];
+      v += __shfl_xor_sync(0xffffffffu, v, 8);
+      v += __shfl_xor_sync(0xffffffffu, v, 16);
+      if (lane < 8) part[warp][j][c8 * 8 + i] = v;
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256, 3) few_rows_kernel(GroupedArgs a, int slices) {
+  __shared__ float xs[kFewK][kFewRows];
+  __shared__ float part[8][kFewRows][64];
+  __shared__ float sum[kFewRows][64];
+  __shared__ int found;
+  const int lane = lane_id();
+  const uint32_t rank = blockIdx.z;
+  const int R = static_cast<int>(a.R);
+  const GP p{a.offsets, a.G, R};
+  if (threadIdx.x < 32) {  // the blockIdx.y-th group with rows
+    int seen = 0, g = -1;
+    for (int g0 = 0; g0 < a.G && g < 0; g0 += 32) {
+      const int2 r = g0 + lane < a.G ? group_range(p, g0 + lane) : make_int2(0, 0);
+      const unsigned m = __ballot_sync(0xffffffffu, r.y > r.x);
+      const int n = __popc(m), want = static_cast<int>(blockIdx.y) - seen;
+      if (want < n) {  // the want-th set bit: the lane with that many below it
+        const unsigned hit = __ballot_sync(0xffffffffu, r.y > r.x && __popc(m & ((1u << lane) - 1u)) == want);
+        g = g0 + __ffs(hit) - 1;
+      }
+      seen += n;
+    }
+    if (lane == 0) found = g;
+  }
+  if (blockIdx.x == 0 && blockIdx.y == 0 && rank == 0) {
+    for (int g = threadIdx.x; g < a.G; g += 256)
+      if (a.offsets[g] < 0 || a.offsets[g + 1] < a.offsets[g] || a.offsets[g + 1] > R) report_error(a.status, kIndexOutOfRange, g);
+  }
+  if (blockIdx.y == 0 && rank == 0) {  // rows of no group
+    const int first = group_range(p, 0).x, last = group_range(p, a.G - 1).y;
+    for (int i = threadIdx.x; i < R * 64; i += 256) {
+      const int r = i >> 6, c = blockIdx.x * 64 + (i & 63);
+      if ((r < first || r >= last) && c < a.N) store_any(a.out, static_cast<int64_t>(r) * a.N + c, a.out_dtype, 0.f);
+    }
+  }
+  __syncthreads();
+  const int g = found;
+  if (g < 0) return;  // every CTA of the cluster
+  const int2 rg = group_range(p, g);
+  const int per = (a.K + slices - 1) / slices, k0 = min(a.K, static_cast<int>(rank) * per), k1 = min(a.K, k0 + per);
+  for (int r0 = rg.x; r0 < rg.y; r0 += kFewRows) {
+    const int nr = min(kFewRows, rg.y - r0);
+    if (nr == 1) few_rows<T, 1>(a, g, r0, nr, k0, k1, xs, part);
+    else if (nr == 2) few_rows<T, 2>(a, g, r0, nr, k0, k1, xs, part);
+    else few_rows<T, 4>(a, g, r0, nr, k0, k1, xs, part);
+    __syncthreads();
+    for (int i = threadIdx.x; i < nr * 64; i += 256) {
+      float v = 0.f;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v += part[q][i >> 6][i & 63];
+      sum[i >> 6][i & 63] = v;
+    }
+    if (slices > 1) sm100::cluster_sync();
+    else __syncthreads();
+    if (rank == 0) {
+      for (int i = threadIdx.x; i < nr * 64; i += 256) {
+        const int c = blockIdx.x * 64 + (i & 63);
+        if (c >= a.N) continue;
+        float v = sum[i >> 6][i & 63];
+        for (int q = 1; q < slices; ++q) v += cluster_value(&sum[i >> 6][i & 63], q);
+        if (a.bias != nullptr) v += load_any(a.bias, static_cast<int64_t>(g) * a.N + c, a.bias_dtype);
+        store_any(a.out, static_cast<int64_t>(r0 + (i >> 6)) * a.N + c, a.out_dtype, v);
+      }
+    }
+    if (slices > 1) sm100::cluster_sync();  // the sums are read before they are overwritten, or their CTA leaves
+    else __syncthreads();
+  }
+}
+
+// Column slices that fill the machine about twice over: K is cut where groups and columns are few.
+int slices_for(int64_t blocks, int64_t length, int64_t least) {
+  int n = 1;
+  while (n < 8 && blocks * n < 296 && length >= 2 * n * least) n *= 2;
+  return n;
+}
+
+void few_rows_launch(const GroupedArgs& a, cudaStream_t s) {
+  const int groups = static_cast<int>(std::min<int64_t>(a.G, a.R)), cols = ceil_div(a.N, 64);
+  const int slices = slices_for(static_cast<int64_t>(groups) * cols, a.K, 128);
+  const dim3 grid(cols, groups, slices);
+  if (a.dtype == kBF16) launch_cluster(few_rows_kernel<__nv_bfloat16>, grid, 256, slices, s, a, slices);
+  else launch_cluster(few_rows_kernel<__half>, grid, 256, slices, s, a, slices);
 }
 
 // ------------------------------------------------------- per-group column sums
-// Block = 64 columns (eight lanes x 8) of one slice of one group; 32 rows at a time.  The slices'
-// sums are added in order by the second kernel: nothing depends on the schedule.
+// Rows are cut into chunks of equal length whatever the groups' sizes (by group, the fullest one
+// would hold up the others).  Block = 256 columns (a warp reads 512 bytes of a row) of one chunk;
+// each group's part of the chunk is a segment of its own, number chunk + group: one of the two
+// grows from a segment to the next.  The second kernel adds a group's segments in order.
+constexpr int kSumRows = 512;
+
 template <typename T>
-__global__ void __launch_bounds__(256) group_sum_kernel(GroupSumArgs a, float* part, int slices) {
-  const int g = blockIdx.y, sl = blockIdx.z;
-  const int lo = min(max(a.offsets[g], 0), static_cast<int>(a.R)), hi = min(max(a.offsets[g + 1], lo), static_cast<int>(a.R));
-  const int per = (hi - lo + slices - 1) / slices;
-  const int r0 = lo + sl * per, r1 = min(hi, r0 + per);
-  const int c = blockIdx.x * 64 + (threadIdx.x & 7) * 8, rr = threadIdx.x >> 3;
-  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (c < a.N) {
+__global__ void __launch_bounds__(256) group_part_kernel(GroupSumArgs a) {
+  __shared__ float red[8][256];
+  const GP p{a.offsets, a.G, static_cast<int>(a.R)};
+  const int lane = lane_id(), warp = warp_id(), chunk = blockIdx.x;
+  const int c0 = chunk * kSumRows, c1 = min(p.R, c0 + kSumRows), c = blockIdx.y * 256 + lane * 8;
+  int lo = 0, hi = a.G;  // the first group that ends behind c0
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (group_range(p, mid).y > c0) hi = mid;
+    else lo = mid + 1;
+  }
+  for (int g = lo; g < a.G; ++g) {
+    const int2 rg = group_range(p, g);
+    if (rg.x >= c1) break;
+    const int r0 = max(rg.x, c0), r1 = min(rg.y, c1);
+    if (r0 >= r1) continue;
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (c < a.N) {
+#pragma unroll 8
+      for (int r = r0 + warp; r < r1; r += 8) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.y) + r * a.ldy + c));
+        const T* v = reinterpret_cast<const T*>(&u);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] += to_f32(v[i]);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) red[warp][lane * 8 + i] = acc[i];
+    __syncthreads();
+    const int col = blockIdx.y * 256 + threadIdx.x;
+    float v = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v += red[i][threadIdx.x];
+    if (col < a.N) a.work[static_cast<int64_t>(chunk + g) * a.N + col] = v;
+  }
+}
+
+__global__ void __launch_bounds__(256) group_sum_kernel(GroupSumArgs a) {
+  const int g = blockIdx.x, col = blockIdx.y * 256 + threadIdx.x;
+  if (col >= a.N) return;
+  const int2 rg = group_range(GP{a.offsets, a.G, static_cast<int>(a.R)}, g);
+  float v = 0.f;
+  if (rg.y > rg.x) {
 #pragma unroll 4
-    for (int r = r0 + rr; r < r1; r += 32) {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.y) + r * a.ldy + c));
-      const T* v = reinterpret_cast<const T*>(&u);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) acc[i] += to_f32(v[i]);
-    }
+    for (int c = rg.x / kSumRows; c <= (rg.y - 1) / kSumRows; ++c) v += a.work[static_cast<int64_t>(c + g) * a.N + col];
   }
-  __shared__ float red[32][65];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) red[rr][(threadIdx.x & 7) * 8 + i] = acc[i];
-  __syncthreads();
-  if (threadIdx.x < 64) {
-    const int col = blockIdx.x * 64 + threadIdx.x;
-    if (col >= a.N) return;
-    float sum = 0.f;
-    for (int i = 0; i < 32; ++i) sum += red[i][threadIdx.x];
-    if (part != nullptr) {
-      part[(static_cast<int64_t>(g) * slices + sl) * a.N + col] = sum;
-      return;
-    }
-    const int64_t o = static_cast<int64_t>(g) * a.N + col;
-    if (a.out_dtype == kF32) static_cast<float*>(a.out)[o] = a.accumulate ? static_cast<float*>(a.out)[o] + sum : sum;
-    else if (a.out_dtype == kBF16) static_cast<__nv_bfloat16*>(a.out)[o] = __float2bfloat16_rn(sum);
-    else static_cast<__half*>(a.out)[o] = __float2half_rn(sum);
-  }
+  const int64_t o = static_cast<int64_t>(g) * a.N + col;
+  if (a.accumulate) v += static_cast<const float*>(a.out)[o];
+  store_any(a.out, o, a.out_dtype, v);
 }
 
 }  // namespace
@@ -664,6 +931,7 @@ void grouped_gemm(const GroupedArgs& a, cudaStream_t s) {
   FLARE_CHECK(a.G > 0 && a.G <= kGroupedMaxGroups, "grouped products: 1 to 2048 groups");
   FLARE_CHECK(a.K > 0 && a.N > 0 && a.K % 8 == 0 && a.N % 8 == 0, "grouped products: widths must be multiples of 8");
   FLARE_CHECK(a.R >= 0 && a.R < (1ll << 31) - 512 && a.x_rows < (1ll << 31) - 512, "grouped products: too many rows");
+  FLARE_CHECK(a.rows == nullptr || (a.mode == kGroupedFwd && grouped_few_rows(a.R)), "grouped products: rows are gathered beforehand");
   // a thread of the autograd engine may not have the device's context yet, and encoding a tensor map needs one
   int dev = 0;
   FLARE_CUDA_CHECK(cudaGetDevice(&dev));
@@ -671,24 +939,37 @@ void grouped_gemm(const GroupedArgs& a, cudaStream_t s) {
   switch (a.mode) {
     case kGroupedFwd:
       if (a.R == 0) return;
-      a.rows != nullptr ? pick<kGroupedFwd, true>(a, s) : pick<kGroupedFwd, false>(a, s);
+      if (grouped_few_rows(a.R)) few_rows_launch(a, s);
+      else pick<kGroupedFwd>(a, s);
       break;
     case kGroupedDgrad:
       if (a.R == 0) return;
-      pick<kGroupedDgrad, false>(a, s);
+      pick<kGroupedDgrad>(a, s);
       break;
     default:
-      a.rows != nullptr ? pick<kGroupedWgrad, true>(a, s) : pick<kGroupedWgrad, false>(a, s);
+      wgrad(a, s);
       break;
   }
 }
 
+int64_t grouped_work_floats(int G, int64_t R, int K, int N) {
+  const int slices = wgrad_shape(G, R, K, N).slices;
+  return slices > 1 ? static_cast<int64_t>(slices) * G * K * N : 0;
+}
+
+bool grouped_few_rows(int64_t rows) { return rows <= 64; }
+
+int64_t group_sum_work_floats(int G, int64_t R, int N) { return ((R + kSumRows - 1) / kSumRows + G) * N; }
+
 void group_colsum(const GroupSumArgs& a, cudaStream_t s) {
-  const dim3 grid(ceil_div(a.N, 64), a.G, 1);
-  if (a.dtype == kBF16) group_sum_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(a, nullptr, 1);
-  else group_sum_kernel<__half><<<grid, 256, 0, s>>>(a, nullptr, 1);
+  const int cols = ceil_div(a.N, 256);
+  const dim3 grid(ceil_div(a.R, kSumRows), cols);
+  if (a.dtype == kBF16) group_part_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(a);
+  else group_part_kernel<__half><<<grid, 256, 0, s>>>(a);
   FLARE_CUDA_CHECK(cudaGetLastError());
-  count_launch();
+  group_sum_kernel<<<dim3(a.G, cols), 256, 0, s>>>(a);
+  FLARE_CUDA_CHECK(cudaGetLastError());
+  count_launch(2);
 }
 
 }  // namespace flare
