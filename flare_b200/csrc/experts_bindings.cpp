@@ -341,8 +341,12 @@ void group_sums(const Tensor& dy, const Tensor& offsets, const Tensor& db, bool 
   b.out = db.data_ptr();
   b.out_dtype = code_of(db.scalar_type());
   b.accumulate = accumulate ? 1 : 0;
-  const Tensor work = empty({flare::group_sum_work_floats(b.G, b.R, b.N)}, dy, at::kFloat);
-  b.work = work.data_ptr<float>();
+  const int64_t scratch = flare::group_sum_work_floats(b.G, b.R, b.N);
+  Tensor work;
+  if (scratch > 0) {
+    work = empty({scratch}, dy, at::kFloat);
+    b.work = work.data_ptr<float>();
+  }
   if (b.R > 0) flare::group_colsum(b, stream());
   else if (!accumulate) db.zero_();
 }

@@ -15,12 +15,13 @@
 // (TMA, a STAGES-deep ring of 128-byte-swizzled tiles), warp 1 issues the MMAs
 // into one of two TMEM accumulators, warps 2..9 drain the other: the epilogue of
 // a tile overlaps the mainloop of the next (with K = 512 a mainloop is 4096 cycles,
-// and four warps took longer than that to write 256 x 256 values).  The rows of the weight gradient's
-// last, partial step are fetched four at a time by index (a row outside the tensor
-// reads as zeros: the next group's rows, and whatever infinities are in them, never
-// enter a product).  Rows are gathered from the tokens by a kernel of their own
-// before the product: fetched by index inside it, four rows cost 45 ns of a CTA's
-// load unit, 1293 us against 432 us for 131072 x 512 x 4096.
+// and four warps took longer than that to write 256 x 256 values).  The weight
+// gradient's last, partial step of a group multiplies whole sixteens of rows: warp 1
+// of the CTA that staged it overwrites the rows of the next group among them with
+// zeros (whatever infinities are in them never enter a product).  Rows are gathered
+// from the tokens by a kernel of their own before the product: fetched by index
+// inside it (four rows a load), they cost 45 ns of a CTA's load unit each time,
+// 1293 us against 432 us for 131072 x 512 x 4096.
 // Variants: CTA pairs on 256 x 256 tiles (each CTA stages half of B, which halves
 // its operand traffic), one CTA on 128 x 128 or 128 x 64 tiles.
 // Every sum is held in fp32 and rounded once.  Every wait is bounded.
@@ -73,7 +74,7 @@ struct Smem {
   static constexpr int kOffBias = kOffEpi + kEpiWarps * 2048;   // 32 floats per epilogue warp
   static constexpr int kOffPre = kOffBias + kEpiWarps * 128;    // tile prefix of the groups, or their order
   static constexpr int kOffBar = kOffPre + (kGroupedMaxGroups + 2) * 4;
-  static constexpr int kBytes = kOffBar + (2 * STAGES + 4) * 8 + 16;
+  static constexpr int kBytes = kOffBar + (3 * STAGES + 4) * 8 + 16;
   static constexpr int kAlloc = kBytes + 1024;
   static_assert(kOffBar % 8 == 0, "barriers are 8-byte aligned");
   static_assert(kAlloc <= 227 * 1024, "shared memory of one CTA");
@@ -224,10 +225,17 @@ __device__ __forceinline__ void zero_outside(const GP& p, int warp, int warps) {
   }
 }
 
-// ta / tb: tiles of A and B; ga / gb: the same tensors with boxes of one row (rows by index).
+// Zeros in rows [r, r rounded up to 16) of `boxes` MN-major boxes (64 rows of 128 bytes) by one warp.
+__device__ __forceinline__ void zero_rows(uint8_t* tile, int boxes, int r) {
+  const int n = ((r + 15) & ~15) - r;
+  for (int i = lane_id(); i < boxes * n * 8; i += 32) {
+    const int box = i / (n * 8), j = i - box * n * 8;
+    *reinterpret_cast<uint4*>(tile + box * 8192 + r * 128 + j * 16) = make_uint4(0, 0, 0, 0);
+  }
+}
+
 template <int MODE, bool PAIR, int BN, int STAGES>
-__device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& ga,
-                                             const CUtensorMap& gb, const GP& p) {
+__device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtensorMap& tb, const GP& p) {
   using L = Smem<PAIR, BN, STAGES>;
   constexpr int BM = PAIR ? 256 : 128;
   constexpr bool A_MN = MODE == kGroupedWgrad, B_MN = MODE != kGroupedDgrad;
@@ -237,7 +245,8 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
   int* pre = reinterpret_cast<int*>(sm + L::kOffPre);
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + L::kOffBar);
   uint64_t* empty = full + STAGES;
-  uint64_t* acc_full = empty + STAGES;
+  uint64_t* tail = empty + STAGES;  // a partial step has landed in this CTA
+  uint64_t* acc_full = tail + STAGES;
   uint64_t* acc_empty = acc_full + 2;
   uint32_t* slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   const int warp = warp_id(), lane = lane_id();
@@ -250,6 +259,7 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
     for (int s = 0; s < STAGES; ++s) {
       sm100::mbar_init(&full[s], 1);
       sm100::mbar_init(&empty[s], 1);
+      sm100::mbar_init(&tail[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       sm100::mbar_init(&acc_full[b], 1);
@@ -318,89 +328,112 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
-    uint32_t it = 0;
-    bool ok = true;
-    auto load2 = [&](void* dst, const CUtensorMap& m, int s, int x, int y) {
-      if constexpr (PAIR) sm100::tma_load_2d_pair(dst, &m, sm100::mapa_shared(&full[s], 0), x, y);
-      else sm100::tma_load_2d(dst, &m, &full[s], x, y);
-    };
-    auto load3 = [&](void* dst, const CUtensorMap& m, int s, int x, int y, int z) {
-      if constexpr (PAIR) sm100::tma_load_3d_pair(dst, &m, sm100::mapa_shared(&full[s], 0), x, y, z);
-      else sm100::tma_load_3d(dst, &m, &full[s], x, y, z);
-    };
-    auto gather = [&](void* dst, const CUtensorMap& m, int s, int x, int4 r) {
-      if constexpr (PAIR) sm100::tma_gather4_pair(dst, &m, sm100::mapa_shared(&full[s], 0), x, r);
-      else sm100::tma_gather4(dst, &m, &full[s], x, r);
-    };
-    // rows r .. r + 3, a row of zeros in the place of those from hi on
-    auto row4 = [&](int r, int hi) {
-      return make_int4(r < hi ? r : p.R, r + 1 < hi ? r + 1 : p.R, r + 2 < hi ? r + 2 : p.R, r + 3 < hi ? r + 3 : p.R);
-    };
-    while (ok && walk.next(t)) {
-      for (int k = 0; k < t.steps; ++k, ++it) {
-        const int s = it % STAGES;
-        if (it >= STAGES && !sm100::mbar_wait(&empty[s], ((it / STAGES) - 1) & 1, p.timeout_ns, p.status, 400 + s)) ok = false;
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
-        uint8_t* sa = sm + s * kTileA;
-        uint8_t* sb = sm + L::kOffB + s * L::kTileB;
-        if (lane == 0 && rank == 0) sm100::mbar_arrive_expect_tx(&full[s], (PAIR ? 2 : 1) * L::kStage);
-        if constexpr (MODE != kGroupedWgrad) {
-          const int k0 = k * kBK;
-          if (lane == 0) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      auto load2 = [&](void* dst, const CUtensorMap& m, int s, int x, int y) {
+        if constexpr (PAIR) sm100::tma_load_2d_pair(dst, &m, sm100::mapa_shared(&full[s], 0), x, y);
+        else sm100::tma_load_2d(dst, &m, &full[s], x, y);
+      };
+      auto load3 = [&](void* dst, const CUtensorMap& m, int s, int x, int y, int z) {
+        if constexpr (PAIR) sm100::tma_load_3d_pair(dst, &m, sm100::mapa_shared(&full[s], 0), x, y, z);
+        else sm100::tma_load_3d(dst, &m, &full[s], x, y, z);
+      };
+      while (ok && walk.next(t)) {
+        for (int k = 0; k < t.steps; ++k, ++it) {
+          const int s = it % STAGES;
+          if (it >= STAGES && !sm100::mbar_wait(&empty[s], ((it / STAGES) - 1) & 1, p.timeout_ns, p.status, 400 + s)) {
+            ok = false;
+            break;
+          }
+          uint8_t* sa = sm + s * kTileA;
+          uint8_t* sb = sm + L::kOffB + s * L::kTileB;
+          const int nb = t.n0 + rank * L::kBNh;
+          if constexpr (MODE != kGroupedWgrad) {
+            if (rank == 0) sm100::mbar_arrive_expect_tx(&full[s], (PAIR ? 2 : 1) * L::kStage);
+            const int k0 = k * kBK;
             load2(sa, ta, s, k0, t.m0 + rank * 128);
             if constexpr (B_MN) {
 #pragma unroll
-              for (int j = 0; j < L::kBNh / 64; ++j) load3(sb + j * 8192, tb, s, t.n0 + rank * L::kBNh + 64 * j, k0, t.g);
+              for (int j = 0; j < L::kBNh / 64; ++j) load3(sb + j * 8192, tb, s, nb + 64 * j, k0, t.g);
             } else {
-              load3(sb, tb, s, k0, t.n0 + rank * L::kBNh, t.g);
+              load3(sb, tb, s, k0, nb, t.g);
             }
-          }
-        } else {
-          const int r0 = t.lo + k * kBK, ma = t.m0 + rank * 128, nb = t.n0 + rank * L::kBNh;
-          if (r0 + kBK <= t.hi) {
-            if (lane == 0) {
+          } else {
+            const int r0 = t.lo + k * kBK, ma = t.m0 + rank * 128;
+            if (r0 + kBK <= t.hi) {
+              if (rank == 0) sm100::mbar_arrive_expect_tx(&full[s], (PAIR ? 2 : 1) * L::kStage);
               load2(sa, ta, s, ma, r0);
               load2(sa + 8192, ta, s, ma + 64, r0);
 #pragma unroll
               for (int j = 0; j < L::kBNh / 64; ++j) load2(sb + j * 8192, tb, s, nb + 64 * j, r0);
-            }
-          } else {
-            const int sub = lane & 15, half = lane >> 4;
-            const int4 r = row4(r0 + 4 * sub, t.hi);
-            gather(sa + half * 8192 + sub * 512, ga, s, ma + 64 * half, r);
+            } else {
+              sm100::mbar_arrive_expect_tx(&tail[s], L::kStage);
+              sm100::tma_load_2d(sa, &ta, &tail[s], ma, r0);
+              sm100::tma_load_2d(sa + 8192, &ta, &tail[s], ma + 64, r0);
 #pragma unroll
-            for (int j = 0; j < L::kBNh / 64; j += 2)
-              if (j + half < L::kBNh / 64) gather(sb + (j + half) * 8192 + sub * 512, gb, s, nb + 64 * (j + half), r);
+              for (int j = 0; j < L::kBNh / 64; ++j) sm100::tma_load_2d(sb + j * 8192, &tb, &tail[s], nb + 64 * j, r0);
+            }
           }
         }
       }
     }
+    __syncwarp();
   } else if (warp == 1) {
     // ---------------------------------------------------------- MMA issuer
-    if (lane == 0 && rank == 0) {
-      uint32_t it = 0, i = 0;
-      bool ok = true;
-      while (ok && walk.next(t)) {
-        if (t.steps == 0) continue;
-        const int buf = i & 1;
-        const uint32_t d = tmem + buf * BN;
-        if (i >= 2 && !sm100::mbar_wait_cluster(&acc_empty[buf], ((i >> 1) - 1) & 1, p.timeout_ns, p.status, 420 + buf)) break;
-        sm100::tc_fence_after();
-        for (int k = 0; k < t.steps; ++k, ++it) {
-          const int s = it % STAGES;
-          if (!sm100::mbar_wait(&full[s], (it / STAGES) & 1, p.timeout_ns, p.status, 440 + s)) {
+    // The whole warp walks the steps (it writes a partial step's zeros); lane 0 of the even CTA issues.
+    uint32_t it = 0, i = 0, tails = 0;
+    bool ok = true;
+    while (ok && walk.next(t)) {
+      if (t.steps == 0) continue;
+      const int buf = i & 1;
+      const uint32_t d = tmem + buf * BN;
+      const int last = MODE == kGroupedWgrad ? (t.hi - t.lo) - (t.steps - 1) * kBK : kBK;  // rows of the last step
+      if (rank == 0 && i >= 2 &&
+          !sm100::mbar_wait_cluster(&acc_empty[buf], ((i >> 1) - 1) & 1, p.timeout_ns, p.status, 420 + buf))
+        ok = false;
+      if (!__all_sync(0xffffffffu, ok)) break;
+      sm100::tc_fence_after();
+      for (int k = 0; k < t.steps; ++k, ++it) {
+        const int s = it % STAGES;
+        uint8_t* sa = sm + s * kTileA;
+        uint8_t* sb = sm + L::kOffB + s * L::kTileB;
+        int sixteens = kBK / 16;
+        if (MODE == kGroupedWgrad && k == t.steps - 1 && last < kBK) {
+          if (!sm100::mbar_wait(&tail[s], (tails >> s) & 1, p.timeout_ns, p.status, 480 + s)) ok = false;
+          tails ^= 1u << s;
+          if (!__all_sync(0xffffffffu, ok)) {
             ok = false;
             break;
           }
+          zero_rows(sa, 2, last);
+          zero_rows(sb, L::kBNh / 64, last);
+          sm100::fence_proxy_async_smem();
+          __syncwarp();
+          sixteens = (last + 15) / 16;
+          // the pair's step is complete when the odd CTA says so; a CTA of its own says so itself
+          if (lane == 0) {
+            if constexpr (PAIR) {
+              if (rank == 1) sm100::mbar_arrive_cluster(sm100::mapa_shared(&full[s], 0));
+            } else {
+              sm100::mbar_arrive(&full[s]);
+            }
+          }
+        }
+        if (rank != 0) continue;
+        if (!sm100::mbar_wait_cluster(&full[s], (it / STAGES) & 1, p.timeout_ns, p.status, 440 + s)) ok = false;
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) {
           sm100::tc_fence_after();
-          const uint32_t sa = smem_u32(sm + s * kTileA), sb = smem_u32(sm + L::kOffB + s * L::kTileB);
+          const uint32_t a0 = smem_u32(sa), b0 = smem_u32(sb);
 #pragma unroll
           for (int q = 0; q < kBK / 16; ++q) {
-            const uint64_t da = A_MN ? sm100::make_smem_desc(sa + q * 2048, 8192, 1024) : sm100::make_smem_desc(sa + q * 32, 16, 1024);
-            const uint64_t db = B_MN ? sm100::make_smem_desc(sb + q * 2048, 8192, 1024) : sm100::make_smem_desc(sb + q * 32, 16, 1024);
+            if (MODE == kGroupedWgrad && q >= sixteens) break;
+            const uint64_t da = A_MN ? sm100::make_smem_desc(a0 + q * 2048, 8192, 1024) : sm100::make_smem_desc(a0 + q * 32, 16, 1024);
+            const uint64_t db = B_MN ? sm100::make_smem_desc(b0 + q * 2048, 8192, 1024) : sm100::make_smem_desc(b0 + q * 32, 16, 1024);
             if constexpr (PAIR) sm100::mma_f16_ss_pair(d, da, db, p.idesc, (k | q) != 0);
             else sm100::mma_f16_ss(d, da, db, p.idesc, (k | q) != 0);
           }
@@ -411,17 +444,19 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
             sm100::mma_commit(&empty[s]);
           }
         }
-        if (!ok) break;
+        __syncwarp();
+      }
+      if (ok && rank == 0 && lane == 0) {
         if constexpr (PAIR) {
           sm100::mma_commit_pair(sm100::mapa_shared(&acc_full[buf], 0));
           sm100::mma_commit_pair(sm100::mapa_shared(&acc_full[buf], 1));
         } else {
           sm100::mma_commit(&acc_full[buf]);
         }
-        ++i;
       }
+      __syncwarp();
+      ++i;
     }
-    __syncwarp();
   } else {
     // ------------------------------------------------------------ epilogue
     const int quarter = warp & 3;  // the TMEM lanes that this warp may read
@@ -437,13 +472,21 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
       const int rows = min(32, (MODE == kGroupedWgrad ? p.Mo : t.hi) - row0);
       const int chunks = rows > 0 ? min(BN / 64, (p.No - t.n0 - c0 + 31) / 32) : 0;  // of 32 columns, with some inside
       const int64_t base = MODE == kGroupedWgrad ? (static_cast<int64_t>(t.slice) * p.G + t.g) * p.Mo * p.ldo : 0;
-      auto finish = [&](uint32_t (&r)[32], int c) {
+      float ahead[BN / 64];  // this lane's column of each chunk: asked for before the products are done
+      if (MODE == kGroupedFwd && p.bias != nullptr) {
+#pragma unroll
+        for (int c = 0; c < BN / 64; ++c) {
+          const int col = t.n0 + c0 + c * 32 + lane;
+          ahead[c] = col < p.No ? load_any(p.bias, static_cast<int64_t>(t.g) * p.No + col, p.bias_dtype) : 0.f;
+        }
+      }
+      auto finish = [&](uint32_t (&r)[32], int c, float b0) {
         const int col = t.n0 + c0 + c * 32;
         float v[32];
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
         if (MODE == kGroupedFwd && p.bias != nullptr) {
-          bias[lane] = col + lane < p.No ? load_any(p.bias, static_cast<int64_t>(t.g) * p.No + col + lane, p.bias_dtype) : 0.f;
+          bias[lane] = b0;
           __syncwarp();
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
@@ -460,16 +503,18 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
         const uint32_t at = tmem + buf * BN + c0 + (static_cast<uint32_t>(quarter * 32) << 16);
         uint32_t ra[32], rb[32];  // the next chunk is on its way while one is written
         if (chunks > 0) sm100::tmem_ld_32x32b_x32(at, ra);
-        for (int c = 0; c < chunks; c += 2) {
+#pragma unroll
+        for (int c = 0; c < BN / 64; c += 2) {
+          if (c >= chunks) break;
           sm100::tmem_ld_wait();
           regs_ready(ra);
           if (c + 1 < chunks) sm100::tmem_ld_32x32b_x32(at + (c + 1) * 32, rb);
-          finish(ra, c);
-          if (c + 1 < chunks) {
+          finish(ra, c, ahead[c]);
+          if (c + 1 < BN / 64 && c + 1 < chunks) {
             sm100::tmem_ld_wait();
             regs_ready(rb);
             if (c + 2 < chunks) sm100::tmem_ld_32x32b_x32(at + (c + 2) * 32, ra);
-            finish(rb, c + 1);
+            finish(rb, c + 1, ahead[c + 1 < BN / 64 ? c + 1 : c]);
           }
         }
         sm100::tc_fence_before();
@@ -483,7 +528,7 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
         uint32_t zero[32];
 #pragma unroll
         for (int j = 0; j < 32; ++j) zero[j] = 0u;
-        for (int c = 0; c < chunks; ++c) finish(zero, c);
+        for (int c = 0; c < chunks; ++c) finish(zero, c, 0.f);
       }
     }
   }
@@ -498,16 +543,14 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
 
 template <int MODE, int BN, int STAGES>
 __global__ void __launch_bounds__(kThreads, 1)
-    grouped_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
-                   const __grid_constant__ CUtensorMap ga, const __grid_constant__ CUtensorMap gb, const __grid_constant__ GP p) {
-  grouped_body<MODE, false, BN, STAGES>(ta, tb, ga, gb, p);
+    grouped_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, const __grid_constant__ GP p) {
+  grouped_body<MODE, false, BN, STAGES>(ta, tb, p);
 }
 template <int MODE, int BN, int STAGES>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     grouped_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
-                        const __grid_constant__ CUtensorMap ga, const __grid_constant__ CUtensorMap gb,
                         const __grid_constant__ GP p) {
-  grouped_body<MODE, true, BN, STAGES>(ta, tb, ga, gb, p);
+  grouped_body<MODE, true, BN, STAGES>(ta, tb, p);
 }
 
 // ------------------------------------------------------------------- host
@@ -593,20 +636,16 @@ void launch(const GroupedArgs& a, cudaStream_t s, int slices = 1) {
   p.idesc = sm100::make_idesc_16bit(BM, BN, MODE == kGroupedWgrad, MODE != kGroupedDgrad, a.dtype == kBF16);
   p.status = a.status;
   p.timeout_ns = a.timeout_ns;
-  CUtensorMap ta, tb, ga, gb;
+  CUtensorMap ta, tb;
   if (MODE == kGroupedWgrad) {
     ta = map2(a.x, a.dtype, a.K, a.R, a.ldx, kBK);
-    ga = map2(a.x, a.dtype, a.K, a.R, a.ldx, 1);
     tb = map2(a.dy, a.dtype, a.N, a.R, a.lddy, kBK);
-    gb = map2(a.dy, a.dtype, a.N, a.R, a.lddy, 1);
   } else {
     const int64_t wd[3] = {a.N, a.K, a.G}, wp[2] = {a.N, static_cast<int64_t>(a.K) * a.N};
     const int box_fwd[3] = {64, kBK, 1}, box_bwd[3] = {64, L::kBNh, 1};
     tb = make_map(a.w, a.dtype, 3, wd, wp, MODE == kGroupedFwd ? box_fwd : box_bwd);
     if (MODE == kGroupedFwd) ta = map2(a.x, a.dtype, a.K, a.R, a.ldx, 128);
     else ta = map2(a.dy, a.dtype, a.N, a.R, a.lddy, 128);
-    ga = ta;
-    gb = tb;
   }
   // as many tiles as there can be: the groups' sizes are on the device
   const int64_t tiles = MODE == kGroupedWgrad
@@ -617,11 +656,11 @@ void launch(const GroupedArgs& a, cudaStream_t s, int slices = 1) {
   if constexpr (PAIR) {
     auto kern = grouped_pair_kernel<MODE, BN, STAGES>;
     const int n = static_cast<int>(std::min<int64_t>(std::max<int64_t>(1, tiles), resident(reinterpret_cast<const void*>(kern), L::kAlloc, true, cache)));
-    kern<<<2 * n, kThreads, L::kAlloc, s>>>(ta, tb, ga, gb, p);
+    kern<<<2 * n, kThreads, L::kAlloc, s>>>(ta, tb, p);
   } else {
     auto kern = grouped_kernel<MODE, BN, STAGES>;
     const int n = static_cast<int>(std::min<int64_t>(std::max<int64_t>(1, tiles), resident(reinterpret_cast<const void*>(kern), L::kAlloc, false, cache)));
-    kern<<<n, kThreads, L::kAlloc, s>>>(ta, tb, ga, gb, p);
+    kern<<<n, kThreads, L::kAlloc, s>>>(ta, tb, p);
   }
   FLARE_CUDA_CHECK(cudaGetLastError());
   count_launch();
@@ -865,18 +904,68 @@ void few_rows_launch(const GroupedArgs& a, cudaStream_t s) {
 }
 
 // ------------------------------------------------------- per-group column sums
-// Rows are cut into chunks of equal length whatever the groups' sizes (by group, the fullest one
-// would hold up the others).  Block = 256 columns (a warp reads 512 bytes of a row) of one chunk;
-// each group's part of the chunk is a segment of its own, number chunk + group: one of the two
-// grows from a segment to the next.  The second kernel adds a group's segments in order.
-constexpr int kSumRows = 512;
+// Many rows: rows are cut into chunks of equal length whatever the groups' sizes (by group, the
+// fullest one holds up the others: 517 us against 173 us for 131072 x 4096 in 32 groups).  Block =
+// 256 columns (a warp reads 512 bytes of a row) of one chunk; each group's part of the chunk is a
+// segment of its own, number chunk + group: one of the two grows from a segment to the next.  A
+// second kernel adds a group's segments in order.
+// Up to kSumOneLaunch rows: one kernel, block = 64 columns of a slice of one group, slices of a
+// group a cluster, added in order.
+constexpr int64_t kSumOneLaunch = 8192;
+int sum_rows(int64_t R, int cols) {  // about eight blocks for each SM
+  return static_cast<int>(std::max<int64_t>(32, std::min<int64_t>(512, R * cols / 1184 / 32 * 32)));
+}
 
 template <typename T>
-__global__ void __launch_bounds__(256) group_part_kernel(GroupSumArgs a) {
+__global__ void __launch_bounds__(256) group_sum_small_kernel(GroupSumArgs a, int slices) {
+  __shared__ float red[8][64];
+  __shared__ float sum[64];
+  const int g = blockIdx.y, lane = lane_id(), warp = warp_id(), c8 = threadIdx.x & 7;
+  const uint32_t rank = blockIdx.z;
+  const int2 rg = group_range(GP{a.offsets, a.G, static_cast<int>(a.R)}, g);
+  const int per = (rg.y - rg.x + slices - 1) / slices;
+  const int r0 = min(rg.y, rg.x + static_cast<int>(rank) * per), r1 = min(rg.y, r0 + per);
+  const int c = blockIdx.x * 64 + c8 * 8;
+  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (c < a.N) {
+#pragma unroll 8
+    for (int r = r0 + (threadIdx.x >> 3); r < r1; r += 32) {
+      const uint4 u = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.y) + r * a.ldy + c));
+      const T* v = reinterpret_cast<const T*>(&u);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] += to_f32(v[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 8);
+    acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 16);
+    if (lane < 8) red[warp][c8 * 8 + i] = acc[i];
+  }
+  __syncthreads();
+  float v = 0.f;
+  if (threadIdx.x < 64) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v += red[i][threadIdx.x];
+    sum[threadIdx.x] = v;
+  }
+  if (slices > 1) sm100::cluster_sync();
+  const int col = blockIdx.x * 64 + threadIdx.x;
+  if (rank == 0 && threadIdx.x < 64 && col < a.N) {
+    for (int q = 1; q < slices; ++q) v += cluster_value(&sum[threadIdx.x], q);
+    const int64_t o = static_cast<int64_t>(g) * a.N + col;
+    if (a.accumulate) v += static_cast<const float*>(a.out)[o];
+    store_any(a.out, o, a.out_dtype, v);
+  }
+  if (slices > 1) sm100::cluster_sync();
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) group_part_kernel(GroupSumArgs a, int rows) {
   __shared__ float red[8][256];
   const GP p{a.offsets, a.G, static_cast<int>(a.R)};
   const int lane = lane_id(), warp = warp_id(), chunk = blockIdx.x;
-  const int c0 = chunk * kSumRows, c1 = min(p.R, c0 + kSumRows), c = blockIdx.y * 256 + lane * 8;
+  const int c0 = chunk * rows, c1 = min(p.R, c0 + rows), c = blockIdx.y * 256 + lane * 8;
   int lo = 0, hi = a.G;  // the first group that ends behind c0
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
@@ -910,14 +999,14 @@ __global__ void __launch_bounds__(256) group_part_kernel(GroupSumArgs a) {
   }
 }
 
-__global__ void __launch_bounds__(256) group_sum_kernel(GroupSumArgs a) {
+__global__ void __launch_bounds__(256) group_sum_kernel(GroupSumArgs a, int rows) {
   const int g = blockIdx.x, col = blockIdx.y * 256 + threadIdx.x;
   if (col >= a.N) return;
   const int2 rg = group_range(GP{a.offsets, a.G, static_cast<int>(a.R)}, g);
   float v = 0.f;
   if (rg.y > rg.x) {
 #pragma unroll 4
-    for (int c = rg.x / kSumRows; c <= (rg.y - 1) / kSumRows; ++c) v += a.work[static_cast<int64_t>(c + g) * a.N + col];
+    for (int c = rg.x / rows; c <= (rg.y - 1) / rows; ++c) v += a.work[static_cast<int64_t>(c + g) * a.N + col];
   }
   const int64_t o = static_cast<int64_t>(g) * a.N + col;
   if (a.accumulate) v += static_cast<const float*>(a.out)[o];
@@ -959,15 +1048,24 @@ int64_t grouped_work_floats(int G, int64_t R, int K, int N) {
 
 bool grouped_few_rows(int64_t rows) { return rows <= 64; }
 
-int64_t group_sum_work_floats(int G, int64_t R, int N) { return ((R + kSumRows - 1) / kSumRows + G) * N; }
+int64_t group_sum_work_floats(int G, int64_t R, int N) {
+  return R <= kSumOneLaunch ? 0 : (ceil_div(R, sum_rows(R, ceil_div(N, 256))) + static_cast<int64_t>(G)) * N;
+}
 
 void group_colsum(const GroupSumArgs& a, cudaStream_t s) {
-  const int cols = ceil_div(a.N, 256);
-  const dim3 grid(ceil_div(a.R, kSumRows), cols);
-  if (a.dtype == kBF16) group_part_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(a);
-  else group_part_kernel<__half><<<grid, 256, 0, s>>>(a);
+  if (a.R <= kSumOneLaunch) {
+    const int cols = ceil_div(a.N, 64), slices = slices_for(static_cast<int64_t>(a.G) * cols, a.R / a.G, 128);
+    const dim3 grid(cols, a.G, slices);
+    if (a.dtype == kBF16) launch_cluster(group_sum_small_kernel<__nv_bfloat16>, grid, 256, slices, s, a, slices);
+    else launch_cluster(group_sum_small_kernel<__half>, grid, 256, slices, s, a, slices);
+    return;
+  }
+  const int cols = ceil_div(a.N, 256), rows = sum_rows(a.R, cols);
+  const dim3 grid(ceil_div(a.R, rows), cols);
+  if (a.dtype == kBF16) group_part_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(a, rows);
+  else group_part_kernel<__half><<<grid, 256, 0, s>>>(a, rows);
   FLARE_CUDA_CHECK(cudaGetLastError());
-  group_sum_kernel<<<dim3(a.G, cols), 256, 0, s>>>(a);
+  group_sum_kernel<<<dim3(a.G, cols), 256, 0, s>>>(a, rows);
   FLARE_CUDA_CHECK(cudaGetLastError());
   count_launch(2);
 }
