@@ -26,34 +26,34 @@ namespace {
 constexpr int kSub = 256;  // tokens that are ranked together (one bit each)
 
 // An unsigned key in the order of the logits: NaN above all, -0 equal to +0, -inf at kDeadKey.
+// Adding +0 turns -0 into +0 and every NaN into the positive one, whose key is the largest.
 constexpr uint32_t kDeadKey = 0x007FFFFFu;
 __device__ __forceinline__ uint32_t order_key(float v) {
-  if (v != v) return 0xFFFFFFFFu;
-  const uint32_t b = v == 0.f ? 0u : __float_as_uint(v);
-  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+  const uint32_t b = __float_as_uint(__fadd_rn(v, 0.f));
+  return b ^ (static_cast<uint32_t>(static_cast<int>(b) >> 31) | 0x80000000u);
 }
 
 __device__ __forceinline__ float key_value(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? k & 0x7FFFFFFFu : ~k);
 }
 
-// LANES lanes share a token, each with NV of its experts (expert = v * LANES + lane); 0 is below
-// every logit's key.
+// LANES lanes share a token, each with NV of its experts (expert = v * LANES + lane).
 template <typename T, int LANES, int NV>
-__device__ __forceinline__ void route_load(const RouteParams& p, int slot, int b, bool live, uint32_t (&key)[NV]) {
+__device__ __forceinline__ void route_load(const RouteParams& p, int slot, int b, bool live, T (&raw)[NV]) {
   const int sub = threadIdx.x % LANES;
-  const T* row = static_cast<const T*>(p.logits) + slot * p.stride_slot + b * p.stride_token;
+  const T* row = static_cast<const T*>(p.logits) + slot * p.stride_slot + b * p.stride_token + sub;
 #pragma unroll
-  for (int v = 0; v < NV; ++v) {
-    const int e = v * LANES + sub;
-    key[v] = live && e < p.E ? order_key(to_f32(row[e])) : 0u;
-  }
+  for (int v = 0; v < NV; ++v)
+    if (live && v * LANES + sub < p.E) raw[v] = row[v * LANES];
 }
 
-template <int LANES, int NV>
-__device__ __forceinline__ void route_pick(const RouteParams& p, int slot, int b, bool live_token, uint32_t (&key)[NV],
+template <typename T, int LANES, int NV>
+__device__ __forceinline__ void route_pick(const RouteParams& p, int slot, int b, bool live_token, const T (&raw)[NV],
                                            int* hist) {
   const int sub = threadIdx.x % LANES;
+  uint32_t key[NV];  // 0 is below every logit's key
+#pragma unroll
+  for (int v = 0; v < NV; ++v) key[v] = live_token && v * LANES + sub < p.E ? order_key(to_f32(raw[v])) : 0u;
   int my_e = -1;  // lane j of the token keeps choice j
   uint32_t my_k = kDeadKey;
   for (int j = 0; j < p.k; ++j) {
@@ -99,14 +99,14 @@ __device__ __forceinline__ void route_pick_chunk(const RouteParams& p, int slot,
   for (int e = threadIdx.x; e < p.E; e += blockDim.x) hist[e] = 0;
   __syncthreads();
   const int per = blockDim.x / LANES, mine = b0 + threadIdx.x / LANES;
-  uint32_t key[NV], next[NV];
-  route_load<T, LANES, NV>(p, slot, mine, mine < b1, key);
+  T raw[NV], next[NV];
+  route_load<T, LANES, NV>(p, slot, mine, mine < b1, raw);
   for (int b = b0; b < b1; b += per) {  // block-uniform: the picks shuffle across whole warps
     const int at = mine + b - b0;
     route_load<T, LANES, NV>(p, slot, at + per, at + per < b1, next);
-    route_pick<LANES, NV>(p, slot, at, at < b1, key, hist);
+    route_pick<T, LANES, NV>(p, slot, at, at < b1, raw, hist);
 #pragma unroll
-    for (int v = 0; v < NV; ++v) key[v] = next[v];
+    for (int v = 0; v < NV; ++v) raw[v] = next[v];
   }
   __syncthreads();
 }
@@ -309,63 +309,73 @@ struct alignas(sizeof(T) * N) Vec {
 template <typename T, int N>
 __device__ __forceinline__ void load_f(const T* p, float (&f)[N]) {
   const Vec<T, N> u = *reinterpret_cast<const Vec<T, N>*>(p);
+  if constexpr (sizeof(T) == 2 && N % 2 == 0) {  // in pairs
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&u);
 #pragma unroll
-  for (int i = 0; i < N; ++i) f[i] = to_f32(u.v[i]);
+    for (int i = 0; i < N; i += 2) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        f[i] = __uint_as_float(w[i / 2] << 16);
+        f[i + 1] = __uint_as_float(w[i / 2] & 0xFFFF0000u);
+      } else {
+        const float2 t = __half22float2(*reinterpret_cast<const __half2*>(w + i / 2));
+        f[i] = t.x;
+        f[i + 1] = t.y;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = to_f32(u.v[i]);
+  }
 }
 template <typename T, int N>
 __device__ __forceinline__ void store_f(T* p, const float (&f)[N]) {
   Vec<T, N> u;
+  if constexpr (sizeof(T) == 2 && N % 2 == 0) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(&u);
 #pragma unroll
-  for (int i = 0; i < N; ++i) u.v[i] = from_f32<T>(f[i]);
+    for (int i = 0; i < N; i += 2) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const __nv_bfloat162 t = __floats2bfloat162_rn(f[i], f[i + 1]);
+        w[i / 2] = *reinterpret_cast<const uint32_t*>(&t);
+      } else {
+        const __half2 t = __floats2half2_rn(f[i], f[i + 1]);
+        w[i / 2] = *reinterpret_cast<const uint32_t*>(&t);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) u.v[i] = from_f32<T>(f[i]);
+  }
   *reinterpret_cast<Vec<T, N>*>(p) = u;
 }
 
 // d logits[t, e] = w_j (dw_j - sum_i w_i dw_i) where choice j of t is e, else 0.  A block takes
-// kBwdTokens tokens: a thread works out one token's k values, then all write the rows, which are
-// mostly zeros, in vectors of N.
-constexpr int kBwdTokens = 64;
-template <typename T, int N>
-__global__ void __launch_bounds__(256) route_bwd_kernel(RouteBwdParams p) {
-  extern __shared__ int ex[];  // [kBwdTokens][k], then the values
-  float* g = reinterpret_cast<float*>(ex + kBwdTokens * p.k);
+// kBwdTokens tokens: it writes zeros over their rows in 16-byte stores, then a thread works out
+// one token's k values and puts them in place (the barrier orders the two).
+constexpr int kBwdTokens = 128;
+template <typename T>
+__global__ void __launch_bounds__(kBwdTokens) route_bwd_kernel(RouteBwdParams p) {
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * kBwdTokens;
   const int n = static_cast<int>(min(static_cast<long long>(kBwdTokens), static_cast<long long>(p.T - t0)));
-  for (int i = threadIdx.x; i < n * p.k; i += 256) {
-    ex[i] = p.experts[t0 * p.k + i];
-    g[i] = ex[i] >= 0 ? p.weights[t0 * p.k + i] * p.dweights[t0 * p.k + i] : 0.f;
-  }
+  T* out = static_cast<T*>(p.dlogits) + t0 * p.E;  // 16-byte aligned: kBwdTokens is a multiple of 8
+  constexpr int per = 16 / sizeof(T);
+  const int total = n * p.E, whole = total / per;
+  for (int i = threadIdx.x; i < whole; i += kBwdTokens) reinterpret_cast<uint4*>(out)[i] = make_uint4(0, 0, 0, 0);
+  for (int i = whole * per + threadIdx.x; i < total; i += kBwdTokens) out[i] = from_f32<T>(0.f);
   __syncthreads();
-  if (threadIdx.x < n) {
-    const int i0 = threadIdx.x * p.k;
-    float dot = 0.f;
-    for (int j = 0; j < p.k; ++j) dot += g[i0 + j];
-    for (int j = 0; j < p.k; ++j) {
-      const int64_t i = t0 * p.k + i0 + j;
-      g[i0 + j] = ex[i0 + j] >= 0 ? p.weights[i] * (p.dweights[i] - dot) : 0.f;
-    }
-  }
-  __syncthreads();
-  const int per = p.E / N;
-  for (int c = threadIdx.x; c < n * per; c += 256) {
-    const int t = c / per, e0 = (c - t * per) * N;
-    float f[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = 0.f;
-    for (int j = 0; j < p.k; ++j) {
-      const int at = ex[t * p.k + j] - e0;
-      const float v = g[t * p.k + j];
-#pragma unroll
-      for (int i = 0; i < N; ++i) f[i] = at == i ? v : f[i];
-    }
-    store_f<T, N>(static_cast<T*>(p.dlogits) + (t0 + t) * p.E + e0, f);
+  if (static_cast<int>(threadIdx.x) >= n) return;
+  const int64_t i0 = (t0 + threadIdx.x) * p.k;
+  float dot = 0.f;
+  for (int j = 0; j < p.k; ++j) dot += p.experts[i0 + j] >= 0 ? p.weights[i0 + j] * p.dweights[i0 + j] : 0.f;
+  for (int j = 0; j < p.k; ++j) {
+    const int e = p.experts[i0 + j];
+    if (e >= 0) out[threadIdx.x * p.E + e] = from_f32<T>(p.weights[i0 + j] * (p.dweights[i0 + j] - dot));
   }
 }
 
-template <typename T, int N>
+template <typename T>
 void route_bwd_launch(const RouteBwdParams& p, cudaStream_t s) {
-  const int grid = static_cast<int>((p.T + kBwdTokens - 1) / kBwdTokens), smem = kBwdTokens * p.k * 8;
-  if (p.E % N == 0) route_bwd_kernel<T, N><<<grid, 256, smem, s>>>(p);
-  else route_bwd_kernel<T, 1><<<grid, 256, smem, s>>>(p);
+  route_bwd_kernel<T><<<static_cast<int>((p.T + kBwdTokens - 1) / kBwdTokens), kBwdTokens, 0, s>>>(p);
   FLARE_CUDA_CHECK(cudaGetLastError());
   count_launch();
 }
@@ -412,12 +422,10 @@ __device__ __forceinline__ void pack_e4m3(const float (&v)[N], float inv, bool i
   if constexpr (N == 1) {
     u.v[0] = static_cast<uint8_t>(__nv_cvt_float_to_fp8(v[0] * inv, __NV_SATFINITE, __NV_E4M3));
   } else {
+    uint16_t* w = reinterpret_cast<uint16_t*>(&u);
 #pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const uint16_t two = __nv_cvt_float2_to_fp8x2(make_float2(v[i] * inv, v[i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-      u.v[i] = static_cast<uint8_t>(two & 0xFF);
-      u.v[i + 1] = static_cast<uint8_t>(two >> 8);
-    }
+    for (int i = 0; i < N; i += 2)
+      w[i / 2] = __nv_cvt_float2_to_fp8x2(make_float2(v[i] * inv, v[i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
   }
   if (inf) {
 #pragma unroll
@@ -434,7 +442,7 @@ __device__ __forceinline__ void unpack_e4m3(const uint8_t* in, float scale, floa
   } else {
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
-      const uint16_t two = static_cast<uint16_t>(u.v[i] | (u.v[i + 1] << 8));
+      const uint16_t two = reinterpret_cast<const uint16_t*>(&u)[i / 2];
       const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3)));
       v[i] = f.x * scale;
       v[i + 1] = f.y * scale;
@@ -545,7 +553,7 @@ void swiglu_launch(const SwigluParams& p, bool backward, cudaStream_t s) {
   RowTiling t;
   t.cols = static_cast<int>((p.h + kGroupCols - 1) / kGroupCols) * GL;
   t.rows = t.cols <= 128 ? 256 / t.cols : 1;
-  const int grid = static_cast<int>(std::min<int64_t>((p.R + t.rows - 1) / t.rows, 148 * 16));
+  const int grid = static_cast<int>(std::min<int64_t>((p.R + t.rows - 1) / t.rows, 148 * 64));
   if (!backward) {
     if (p.q != nullptr) swiglu_fwd_kernel<T, N, true><<<grid, 256, 0, s>>>(p, t);
     else swiglu_fwd_kernel<T, N, false><<<grid, 256, 0, s>>>(p, t);
@@ -575,81 +583,109 @@ void swiglu_dispatch(const SwigluParams& p, bool backward, cudaStream_t s) {
 }
 
 // ------------------------------------------------------------- combination
-// A thread owns N columns of one token and reads its k rows one after another (four in flight).
-template <typename T, int N, typename O>
+// A thread owns N columns of two tokens at a time (of one where z is fp32: its registers are full)
+// and reads their rows, KU of each in flight.
+template <typename T, int N, typename O, int KU>
 __global__ void __launch_bounds__(256) combine_fwd_kernel(CombineParams p, RowTiling t) {
+  constexpr int U = sizeof(T) == 2 ? 2 : 1;
   const int r0 = t.rows > 1 ? threadIdx.x / t.cols : 0;
   const int c0 = t.rows > 1 ? threadIdx.x % t.cols : threadIdx.x;
   if (r0 >= t.rows) return;
-  for (int64_t tb = static_cast<int64_t>(blockIdx.x) * t.rows; tb < p.T; tb += static_cast<int64_t>(gridDim.x) * t.rows) {
-    const int64_t tok = tb + r0;
-    if (tok >= p.T) continue;
-    const int* rows = p.row_of + tok * p.k;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * t.rows;
+  for (int64_t tok = static_cast<int64_t>(blockIdx.x) * t.rows + r0; tok < p.T; tok += U * step) {
+    const int live = U == 2 && tok + step < p.T ? 2 : 1;
     for (int c = c0; c < t.cols; c += 256) {
-      float acc[N];
+      const T* z = static_cast<const T*>(p.z) + static_cast<int64_t>(c) * N;
+      float acc[U][N];
 #pragma unroll
-      for (int i = 0; i < N; ++i) acc[i] = 0.f;
-      for (int j0 = 0; j0 < p.k; j0 += 4) {
-        float f[4][N];
-        float w[4];
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int row = j0 + q < p.k ? rows[j0 + q] : -1;
-          w[q] = 0.f;
-          if (row >= 0 && row < p.R) {
-            load_f<T, N>(static_cast<const T*>(p.z) + row * p.ldz + static_cast<int64_t>(c) * N, f[q]);
-            w[q] = p.weights != nullptr ? p.weights[tok * p.k + j0 + q] : 1.f;
-          } else {
+        for (int i = 0; i < N; ++i) acc[u][i] = 0.f;
+      for (int j0 = 0; j0 < p.k; j0 += KU) {
+        int row[U][KU];
+        float w[U][KU], f[U][KU][N];
 #pragma unroll
-            for (int i = 0; i < N; ++i) f[q][i] = 0.f;
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int q = 0; q < KU; ++q) {
+            const int64_t at = (tok + u * step) * p.k + j0 + q;
+            const bool in = u < live && j0 + q < p.k;
+            row[u][q] = in ? p.row_of[at] : -1;
+            w[u][q] = in && p.weights != nullptr ? p.weights[at] : 1.f;
           }
-        }
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-          for (int i = 0; i < N; ++i) acc[i] = fmaf(w[q], f[q][i], acc[i]);
+          for (int q = 0; q < KU; ++q) {
+            if (row[u][q] >= 0 && row[u][q] < p.R) {
+              load_f<T, N>(z + row[u][q] * p.ldz, f[u][q]);
+            } else {
+              w[u][q] = 0.f;
+#pragma unroll
+              for (int i = 0; i < N; ++i) f[u][q][i] = 0.f;
+            }
+          }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int q = 0; q < KU; ++q)
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[u][i] = fmaf(w[u][q], f[u][q][i], acc[u][i]);
       }
-      store_f<O, N>(static_cast<O*>(p.y) + tok * p.N + static_cast<int64_t>(c) * N, acc);
+      O* y = static_cast<O*>(p.y) + static_cast<int64_t>(c) * N;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (u < live) store_f<O, N>(y + (tok + u * step) * p.N, acc[u]);
     }
   }
 }
 
 // A warp per (token, choice): dz[row] = w * dy[t], dw = <z[row], dy[t]>; a token's choices are
-// neighbours, so its dy comes from the caches.  Rows behind the last group get zeros.  Without
-// weights dz[row] = dy[t] and z is not read.
-template <typename T, int N>
+// neighbours, so its dy comes from the caches.  Rows behind the last group get zeros.  kWeighted
+// off: dz[row] = dy[t], and z is not read.
+template <typename T, int N, bool kWeighted>
 __global__ void __launch_bounds__(256) combine_bwd_kernel(CombineParams p) {
   const int lane = lane_id();
   const int64_t warps = static_cast<int64_t>(gridDim.x) * 8, pairs = p.T * p.k;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + warp_id(); i < pairs; i += warps) {
-    const int row = p.row_of[i];
+  int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + warp_id();
+  int next = i < pairs ? p.row_of[i] : -1;  // a pair ahead
+  for (; i < pairs; i += warps) {
+    const int row = next;
+    if (i + warps < pairs) next = p.row_of[i + warps];
     if (row < 0 || row >= p.R) {
-      if (lane == 0 && p.dw != nullptr) p.dw[i] = 0.f;
+      if (kWeighted && lane == 0) p.dw[i] = 0.f;
       continue;
     }
-    const int64_t tok = i / p.k;
-    const float w = p.weights != nullptr ? p.weights[i] : 1.f;
-    const T* dy = static_cast<const T*>(p.dy) + tok * p.lddy;
-    const T* z = static_cast<const T*>(p.z) + row * p.ldz;
+    const float w = kWeighted ? p.weights[i] : 1.f;
+    const T* dy = static_cast<const T*>(p.dy) + (i / p.k) * p.lddy;
+    const T* z = kWeighted ? static_cast<const T*>(p.z) + row * p.ldz : nullptr;
     T* dz = static_cast<T*>(p.dz) + static_cast<int64_t>(row) * p.N;
     float dot = 0.f;
-#pragma unroll 2
-    for (int c = lane * N; c < p.N; c += 32 * N) {
-      float a[N], o[N];
-      load_f<T, N>(dy + c, a);
+    for (int c = lane * N; c < p.N; c += 64 * N) {  // both halves' loads before either store
+      const bool second = c + 32 * N < p.N;
+      float a[2][N], b[2][N];
+      load_f<T, N>(dy + c, a[0]);
+      if (second) load_f<T, N>(dy + c + 32 * N, a[1]);
+      if constexpr (kWeighted) {
+        load_f<T, N>(z + c, b[0]);
+        if (second) load_f<T, N>(z + c + 32 * N, b[1]);
+      }
 #pragma unroll
-      for (int q = 0; q < N; ++q) o[q] = w * a[q];
-      store_f<T, N>(dz + c, o);
-      if (p.dw != nullptr) {
-        float b[N];
-        load_f<T, N>(z + c, b);
+      for (int h = 0; h < 2; ++h) {
+        if (h == 1 && !second) break;
+        float o[N];
 #pragma unroll
-        for (int q = 0; q < N; ++q) dot = fmaf(a[q], b[q], dot);
+        for (int q = 0; q < N; ++q) {
+          if constexpr (kWeighted) dot = fmaf(a[h][q], b[h][q], dot);
+          o[q] = w * a[h][q];
+        }
+        store_f<T, N>(dz + c + h * 32 * N, o);
       }
     }
-    if (p.dw == nullptr) continue;
-    dot = warp_sum(dot);
-    if (lane == 0) p.dw[i] = dot;
+    if constexpr (kWeighted) {
+      dot = warp_sum(dot);
+      if (lane == 0) p.dw[i] = dot;
+    }
   }
   const int64_t total = max(0, *p.total);
   for (int64_t r = total + static_cast<int64_t>(blockIdx.x) * 8 + warp_id(); r < p.R; r += warps) {
@@ -667,16 +703,23 @@ void combine_launch(const CombineParams& p, bool backward, cudaStream_t s) {
     t.cols = p.N / N;
     t.rows = t.cols <= 128 ? 256 / t.cols : 1;
     const int grid = static_cast<int>(std::min<int64_t>((p.T + t.rows - 1) / t.rows, 148 * 16));
+    auto go = [&](auto out) {
+      using O = decltype(out);
+      if (p.k == 1) combine_fwd_kernel<T, N, O, 1><<<grid, 256, 0, s>>>(p, t);
+      else if (p.k == 2) combine_fwd_kernel<T, N, O, 2><<<grid, 256, 0, s>>>(p, t);
+      else combine_fwd_kernel<T, N, O, 4><<<grid, 256, 0, s>>>(p, t);
+    };
     if constexpr (sizeof(T) == 4) {
-      if (p.out_dtype == kBF16) combine_fwd_kernel<T, N, __nv_bfloat16><<<grid, 256, 0, s>>>(p, t);
-      else if (p.out_dtype == kF16) combine_fwd_kernel<T, N, __half><<<grid, 256, 0, s>>>(p, t);
-      else combine_fwd_kernel<T, N, T><<<grid, 256, 0, s>>>(p, t);
+      if (p.out_dtype == kBF16) go(__nv_bfloat16());
+      else if (p.out_dtype == kF16) go(__half());
+      else go(T());
     } else {
-      combine_fwd_kernel<T, N, T><<<grid, 256, 0, s>>>(p, t);
+      go(T());
     }
   } else {
     const int grid = static_cast<int>(std::min<int64_t>((std::max(p.T * p.k, p.R) + 7) / 8, 148 * 16));
-    combine_bwd_kernel<T, N><<<grid, 256, 0, s>>>(p);
+    if (p.weights != nullptr) combine_bwd_kernel<T, N, true><<<grid, 256, 0, s>>>(p);
+    else combine_bwd_kernel<T, N, false><<<grid, 256, 0, s>>>(p);
   }
   FLARE_CUDA_CHECK(cudaGetLastError());
   count_launch();
@@ -714,9 +757,9 @@ void route_topk(const RouteParams& p, cudaStream_t s) {
 void route_topk_backward(const RouteBwdParams& p, cudaStream_t s) {
   if (p.T == 0) return;
   switch (p.dtype) {
-    case kF32: route_bwd_launch<float, 4>(p, s); break;
-    case kBF16: route_bwd_launch<__nv_bfloat16, 8>(p, s); break;
-    default: route_bwd_launch<__half, 8>(p, s); break;
+    case kF32: route_bwd_launch<float>(p, s); break;
+    case kBF16: route_bwd_launch<__nv_bfloat16>(p, s); break;
+    default: route_bwd_launch<__half>(p, s); break;
   }
 }
 

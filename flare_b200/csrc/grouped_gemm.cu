@@ -16,14 +16,16 @@
 // into one of two TMEM accumulators, warps 2..9 drain the other: the epilogue of
 // a tile overlaps the mainloop of the next (with K = 512 a mainloop is 4096 cycles,
 // and four warps took longer than that to write 256 x 256 values).  The weight
-// gradient's last, partial step of a group multiplies whole sixteens of rows: warp 1
-// of the CTA that staged it overwrites the rows of the next group among them with
-// zeros (whatever infinities are in them never enter a product).  Rows are gathered
+// gradient's last, partial step of a group multiplies whole sixteens of rows: a warp
+// overwrites the rows of the next group among them with zeros (whatever infinities
+// are in them never enter a product).  Rows are gathered
 // from the tokens by a kernel of their own before the product: fetched by index
 // inside it (four rows a load), they cost 45 ns of a CTA's load unit each time,
 // 1293 us against 432 us for 131072 x 512 x 4096.
-// Variants: CTA pairs on 256 x 256 tiles (each CTA stages half of B, which halves
-// its operand traffic), one CTA on 128 x 128 or 128 x 64 tiles.
+// Variants: one CTA on 128 x 256, 128 x 128 or 128 x 64 tiles; CTA pairs on 256 x 256
+// tiles (each CTA stages half of B) for long groups.  A tile that reaches past its
+// group loads only the sixteens of rows that the group has: in a serving step that
+// is two of 128.
 // Every sum is held in fp32 and rounded once.  Every wait is bounded.
 #include "experts.cuh"
 #include "gemm.cuh"
@@ -43,7 +45,8 @@ namespace {
 
 constexpr int kBK = 64;          // contraction step: one 128-byte swizzle atom of 16-bit values
 constexpr int kEpiWarps = 8;     // two for each quarter of the TMEM lanes, half of the columns each
-constexpr int kThreads = 64 + 32 * kEpiWarps;  // and the producer and MMA issuer warps
+// the producer and MMA issuer warps, these, and one that zeroes the weight gradient's partial steps
+constexpr int threads_of(int mode) { return 64 + 32 * kEpiWarps + (mode == kGroupedWgrad ? 32 : 0); }
 constexpr int kTileA = 128 * kBK * 2;
 
 struct GP {
@@ -206,6 +209,10 @@ __device__ __forceinline__ void store_chunk(const GP& p, const float (&v)[32], i
   __syncwarp();
 }
 
+// Bytes of A that a CTA loads for the rows from row0 on: one box of 128 rows, or up to four of 16.
+__device__ __forceinline__ int a_boxes(int rows) { return (max(rows, 0) + 15) >> 4; }
+__device__ __forceinline__ uint32_t a_bytes(int rows) { return rows > 64 ? kTileA : a_boxes(rows) * 2048; }
+
 // Keeps uses of a TMEM load's registers behind the wait for it.
 __device__ __forceinline__ void regs_ready(uint32_t (&r)[32]) {
 #pragma unroll
@@ -234,11 +241,14 @@ __device__ __forceinline__ void zero_rows(uint8_t* tile, int boxes, int r) {
   }
 }
 
+// ta / tb: tiles of A and B; ta16: A in boxes of 16 rows (forward, input gradient).
 template <int MODE, bool PAIR, int BN, int STAGES>
-__device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtensorMap& tb, const GP& p) {
+__device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtensorMap& ta16, const CUtensorMap& tb,
+                                             const GP& p) {
   using L = Smem<PAIR, BN, STAGES>;
   constexpr int BM = PAIR ? 256 : 128;
   constexpr bool A_MN = MODE == kGroupedWgrad, B_MN = MODE != kGroupedDgrad;
+  static_assert(!(PAIR && MODE == kGroupedWgrad), "the weight gradient's tiles are one CTA's");
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* sm = smem_raw + (((raw + 1023u) & ~1023u) - raw);
@@ -277,7 +287,7 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
     }
   }
   if constexpr (MODE != kGroupedWgrad) {
-    for (int g = threadIdx.x; g < p.G; g += kThreads) {
+    for (int g = threadIdx.x; g < p.G; g += threads_of(MODE)) {
       const int2 r = group_range(p, g);
       pre[g + 1] = (r.y - r.x + BM - 1) / BM;
     }
@@ -300,12 +310,12 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
   if constexpr (MODE == kGroupedWgrad) {
     if (p.G <= kSortGroups) {  // by falling size, equal ones in order
       int* size = pre + kSortGroups;
-      for (int g = threadIdx.x; g < p.G; g += kThreads) {
+      for (int g = threadIdx.x; g < p.G; g += threads_of(MODE)) {
         const int2 r = group_range(p, g);
         size[g] = r.y - r.x;
       }
       __syncthreads();
-      for (int g = threadIdx.x; g < p.G; g += kThreads) {
+      for (int g = threadIdx.x; g < p.G; g += threads_of(MODE)) {
         const int mine = size[g];
         int at = 0;
         for (int o = 0; o < p.G; ++o) at += size[o] > mine || (size[o] == mine && o < g);
@@ -314,7 +324,7 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
     }
   }
   if (blockIdx.x == 0) {  // a group that ends before it starts, or outside the rows, is reported
-    for (int g = threadIdx.x; g < p.G; g += kThreads)
+    for (int g = threadIdx.x; g < p.G; g += threads_of(MODE))
       if (p.offsets[g] < 0 || p.offsets[g + 1] < p.offsets[g] || p.offsets[g + 1] > p.R)
         report_error(p.status, kIndexOutOfRange, g);
   }
@@ -350,9 +360,14 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
           uint8_t* sb = sm + L::kOffB + s * L::kTileB;
           const int nb = t.n0 + rank * L::kBNh;
           if constexpr (MODE != kGroupedWgrad) {
-            if (rank == 0) sm100::mbar_arrive_expect_tx(&full[s], (PAIR ? 2 : 1) * L::kStage);
-            const int k0 = k * kBK;
-            load2(sa, ta, s, k0, t.m0 + rank * 128);
+            const int k0 = k * kBK, row0 = t.m0 + rank * 128, rows = t.hi - row0;
+            if (rank == 0)
+              sm100::mbar_arrive_expect_tx(&full[s], a_bytes(rows) + L::kTileB + (PAIR ? a_bytes(rows - 128) + L::kTileB : 0));
+            if (rows > 64) {
+              load2(sa, ta, s, k0, row0);
+            } else {
+              for (int j = 0; j < a_boxes(rows); ++j) load2(sa + j * 2048, ta16, s, k0, row0 + j * 16);
+            }
             if constexpr (B_MN) {
 #pragma unroll
               for (int j = 0; j < L::kBNh / 64; ++j) load3(sb + j * 8192, tb, s, nb + 64 * j, k0, t.g);
@@ -360,20 +375,13 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
               load3(sb, tb, s, k0, nb, t.g);
             }
           } else {
-            const int r0 = t.lo + k * kBK, ma = t.m0 + rank * 128;
-            if (r0 + kBK <= t.hi) {
-              if (rank == 0) sm100::mbar_arrive_expect_tx(&full[s], (PAIR ? 2 : 1) * L::kStage);
-              load2(sa, ta, s, ma, r0);
-              load2(sa + 8192, ta, s, ma + 64, r0);
+            const int r0 = t.lo + k * kBK;
+            uint64_t* bar = r0 + kBK <= t.hi ? &full[s] : &tail[s];
+            sm100::mbar_arrive_expect_tx(bar, L::kStage);
+            sm100::tma_load_2d(sa, &ta, bar, t.m0, r0);
+            sm100::tma_load_2d(sa + 8192, &ta, bar, t.m0 + 64, r0);
 #pragma unroll
-              for (int j = 0; j < L::kBNh / 64; ++j) load2(sb + j * 8192, tb, s, nb + 64 * j, r0);
-            } else {
-              sm100::mbar_arrive_expect_tx(&tail[s], L::kStage);
-              sm100::tma_load_2d(sa, &ta, &tail[s], ma, r0);
-              sm100::tma_load_2d(sa + 8192, &ta, &tail[s], ma + 64, r0);
-#pragma unroll
-              for (int j = 0; j < L::kBNh / 64; ++j) sm100::tma_load_2d(sb + j * 8192, &tb, &tail[s], nb + 64 * j, r0);
-            }
+            for (int j = 0; j < L::kBNh / 64; ++j) sm100::tma_load_2d(sb + j * 8192, &tb, bar, nb + 64 * j, r0);
           }
         }
       }
@@ -381,81 +389,69 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
     __syncwarp();
   } else if (warp == 1) {
     // ---------------------------------------------------------- MMA issuer
-    // The whole warp walks the steps (it writes a partial step's zeros); lane 0 of the even CTA issues.
-    uint32_t it = 0, i = 0, tails = 0;
-    bool ok = true;
-    while (ok && walk.next(t)) {
-      if (t.steps == 0) continue;
-      const int buf = i & 1;
-      const uint32_t d = tmem + buf * BN;
-      const int last = MODE == kGroupedWgrad ? (t.hi - t.lo) - (t.steps - 1) * kBK : kBK;  // rows of the last step
-      if (rank == 0 && i >= 2 &&
-          !sm100::mbar_wait_cluster(&acc_empty[buf], ((i >> 1) - 1) & 1, p.timeout_ns, p.status, 420 + buf))
-        ok = false;
-      if (!__all_sync(0xffffffffu, ok)) break;
-      sm100::tc_fence_after();
-      for (int k = 0; k < t.steps; ++k, ++it) {
-        const int s = it % STAGES;
-        uint8_t* sa = sm + s * kTileA;
-        uint8_t* sb = sm + L::kOffB + s * L::kTileB;
-        int sixteens = kBK / 16;
-        if (MODE == kGroupedWgrad && k == t.steps - 1 && last < kBK) {
-          if (!sm100::mbar_wait(&tail[s], (tails >> s) & 1, p.timeout_ns, p.status, 480 + s)) ok = false;
-          tails ^= 1u << s;
-          if (!__all_sync(0xffffffffu, ok)) {
+    // One thread (of the even CTA).  What it does between two steps' products is what the tensor
+    // cores may wait for, so the next step's barrier is tried while this one's products are queued,
+    // and descriptors are an addition each.
+    if (lane == 0 && rank == 0) {
+      // 16 columns of a K-major row are 32 bytes, 16 rows of an MN-major box 2048
+      constexpr int kStepA = (A_MN ? 2048 : 32) >> 4, kStepB = (B_MN ? 2048 : 32) >> 4;
+      const uint64_t da0 = sm100::make_smem_desc(smem_u32(sm), A_MN ? 8192 : 16, 1024);
+      const uint64_t db0 = sm100::make_smem_desc(smem_u32(sm + L::kOffB), B_MN ? 8192 : 16, 1024);
+      uint32_t it = 0, i = 0;
+      bool ok = true, ready = false;
+      while (ok && walk.next(t)) {
+        if (t.steps == 0) continue;
+        const int buf = i & 1;
+        const uint32_t d = tmem + buf * BN;
+        const int last = MODE == kGroupedWgrad ? (t.hi - t.lo) - (t.steps - 1) * kBK : kBK;  // rows of the last step
+        if (i >= 2 && !sm100::mbar_wait_cluster(&acc_empty[buf], ((i >> 1) - 1) & 1, p.timeout_ns, p.status, 420 + buf)) break;
+        sm100::tc_fence_after();
+        for (int k = 0; k < t.steps; ++k) {
+          const int s = it % STAGES;
+          if (!ready && !sm100::mbar_wait_cluster(&full[s], (it / STAGES) & 1, p.timeout_ns, p.status, 440 + s)) {
             ok = false;
             break;
           }
-          zero_rows(sa, 2, last);
-          zero_rows(sb, L::kBNh / 64, last);
-          sm100::fence_proxy_async_smem();
-          __syncwarp();
-          sixteens = (last + 15) / 16;
-          // the pair's step is complete when the odd CTA says so; a CTA of its own says so itself
-          if (lane == 0) {
-            if constexpr (PAIR) {
-              if (rank == 1) sm100::mbar_arrive_cluster(sm100::mapa_shared(&full[s], 0));
-            } else {
-              sm100::mbar_arrive(&full[s]);
+          sm100::tc_fence_after();
+          const uint64_t da = da0 + static_cast<uint32_t>(s) * (kTileA >> 4), db = db0 + static_cast<uint32_t>(s) * (L::kTileB >> 4);
+          if (MODE == kGroupedWgrad && k == t.steps - 1 && last <= kBK - 16) {
+            for (int q = 0; q < (last + 15) / 16; ++q) sm100::mma_f16_ss(d, da + q * kStepA, db + q * kStepB, p.idesc, (k | q) != 0);
+          } else {
+#pragma unroll
+            for (int q = 0; q < kBK / 16; ++q) {
+              if constexpr (PAIR) sm100::mma_f16_ss_pair(d, da + q * kStepA, db + q * kStepB, p.idesc, (k | q) != 0);
+              else sm100::mma_f16_ss(d, da + q * kStepA, db + q * kStepB, p.idesc, (k | q) != 0);
             }
           }
+          if constexpr (PAIR) sm100::mma_commit_pair_both(&empty[s]);
+          else sm100::mma_commit(&empty[s]);
+          ++it;
+          ready = sm100::mbar_test_wait_cluster(&full[it % STAGES], (it / STAGES) & 1);
         }
-        if (rank != 0) continue;
-        if (!sm100::mbar_wait_cluster(&full[s], (it / STAGES) & 1, p.timeout_ns, p.status, 440 + s)) ok = false;
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
-        if (lane == 0) {
-          sm100::tc_fence_after();
-          const uint32_t a0 = smem_u32(sa), b0 = smem_u32(sb);
-#pragma unroll
-          for (int q = 0; q < kBK / 16; ++q) {
-            if (MODE == kGroupedWgrad && q >= sixteens) break;
-            const uint64_t da = A_MN ? sm100::make_smem_desc(a0 + q * 2048, 8192, 1024) : sm100::make_smem_desc(a0 + q * 32, 16, 1024);
-            const uint64_t db = B_MN ? sm100::make_smem_desc(b0 + q * 2048, 8192, 1024) : sm100::make_smem_desc(b0 + q * 32, 16, 1024);
-            if constexpr (PAIR) sm100::mma_f16_ss_pair(d, da, db, p.idesc, (k | q) != 0);
-            else sm100::mma_f16_ss(d, da, db, p.idesc, (k | q) != 0);
-          }
-          if constexpr (PAIR) {
-            sm100::mma_commit_pair(sm100::mapa_shared(&empty[s], 0));
-            sm100::mma_commit_pair(sm100::mapa_shared(&empty[s], 1));
-          } else {
-            sm100::mma_commit(&empty[s]);
-          }
-        }
-        __syncwarp();
+        if (!ok) break;
+        if constexpr (PAIR) sm100::mma_commit_pair_both(&acc_full[buf]);
+        else sm100::mma_commit(&acc_full[buf]);
+        ++i;
       }
-      if (ok && rank == 0 && lane == 0) {
-        if constexpr (PAIR) {
-          sm100::mma_commit_pair(sm100::mapa_shared(&acc_full[buf], 0));
-          sm100::mma_commit_pair(sm100::mapa_shared(&acc_full[buf], 1));
-        } else {
-          sm100::mma_commit(&acc_full[buf]);
-        }
-      }
+    }
+    __syncwarp();
+  } else if (MODE == kGroupedWgrad && warp == 2 + kEpiWarps) {
+    // -------------------------------------------------------- partial steps
+    // A stage's partial steps are waited for one after another: this warp completes each one (the
+    // MMAs and the next load wait for it), so it is never a phase behind, nor ahead.
+    uint32_t it = 0, tails = 0;
+    while (MODE == kGroupedWgrad && walk.next(t)) {
+      it += t.steps;
+      const int last = (t.hi - t.lo) - (t.steps - 1) * kBK;
+      if (t.steps == 0 || last == kBK) continue;
+      const int s = (it - 1) % STAGES;
+      if (!__all_sync(0xffffffffu, sm100::mbar_wait(&tail[s], (tails >> s) & 1, p.timeout_ns, p.status, 480 + s))) break;
+      tails ^= 1u << s;
+      zero_rows(sm + s * kTileA, 2, last);
+      zero_rows(sm + L::kOffB + s * L::kTileB, L::kBNh / 64, last);
+      sm100::fence_proxy_async_smem();
       __syncwarp();
-      ++i;
+      if (lane == 0) sm100::mbar_arrive(&full[s]);
     }
   } else {
     // ------------------------------------------------------------ epilogue
@@ -542,15 +538,16 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
 }
 
 template <int MODE, int BN, int STAGES>
-__global__ void __launch_bounds__(kThreads, 1)
-    grouped_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, const __grid_constant__ GP p) {
-  grouped_body<MODE, false, BN, STAGES>(ta, tb, p);
+__global__ void __launch_bounds__(threads_of(MODE), 1)
+    grouped_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap ta16,
+                   const __grid_constant__ CUtensorMap tb, const __grid_constant__ GP p) {
+  grouped_body<MODE, false, BN, STAGES>(ta, ta16, tb, p);
 }
 template <int MODE, int BN, int STAGES>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    grouped_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
-                        const __grid_constant__ GP p) {
-  grouped_body<MODE, true, BN, STAGES>(ta, tb, p);
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE), 1)
+    grouped_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap ta16,
+                        const __grid_constant__ CUtensorMap tb, const __grid_constant__ GP p) {
+  grouped_body<MODE, true, BN, STAGES>(ta, ta16, tb, p);
 }
 
 // ------------------------------------------------------------------- host
@@ -584,7 +581,7 @@ constexpr int kMaxDevices = 64;
 
 // Sets a kernel's shared-memory limit once per device and returns how many CTAs (or pairs) of it
 // the current device runs at once.
-int resident(const void* kern, int smem, bool pair, int (&cache)[kMaxDevices]) {
+int resident(const void* kern, int threads, int smem, bool pair, int (&cache)[kMaxDevices]) {
   static std::mutex mu;
   int dev = 0;
   FLARE_CUDA_CHECK(cudaGetDevice(&dev));
@@ -596,7 +593,7 @@ int resident(const void* kern, int smem, bool pair, int (&cache)[kMaxDevices]) {
     if (pair) {
       cudaLaunchConfig_t cfg{};
       cfg.gridDim = dim3(2);
-      cfg.blockDim = dim3(kThreads);
+      cfg.blockDim = dim3(threads);
       cfg.dynamicSmemBytes = smem;
       cudaLaunchAttribute at[1];
       at[0].id = cudaLaunchAttributeClusterDimension;
@@ -636,16 +633,19 @@ void launch(const GroupedArgs& a, cudaStream_t s, int slices = 1) {
   p.idesc = sm100::make_idesc_16bit(BM, BN, MODE == kGroupedWgrad, MODE != kGroupedDgrad, a.dtype == kBF16);
   p.status = a.status;
   p.timeout_ns = a.timeout_ns;
-  CUtensorMap ta, tb;
+  CUtensorMap ta, ta16, tb;
   if (MODE == kGroupedWgrad) {
     ta = map2(a.x, a.dtype, a.K, a.R, a.ldx, kBK);
     tb = map2(a.dy, a.dtype, a.N, a.R, a.lddy, kBK);
+    ta16 = ta;
   } else {
     const int64_t wd[3] = {a.N, a.K, a.G}, wp[2] = {a.N, static_cast<int64_t>(a.K) * a.N};
     const int box_fwd[3] = {64, kBK, 1}, box_bwd[3] = {64, L::kBNh, 1};
     tb = make_map(a.w, a.dtype, 3, wd, wp, MODE == kGroupedFwd ? box_fwd : box_bwd);
-    if (MODE == kGroupedFwd) ta = map2(a.x, a.dtype, a.K, a.R, a.ldx, 128);
-    else ta = map2(a.dy, a.dtype, a.N, a.R, a.lddy, 128);
+    const void* rows = MODE == kGroupedFwd ? a.x : a.dy;
+    const int64_t ld = MODE == kGroupedFwd ? a.ldx : a.lddy;
+    ta = map2(rows, a.dtype, p.Kc, a.R, ld, 128);
+    ta16 = map2(rows, a.dtype, p.Kc, a.R, ld, 16);
   }
   // as many tiles as there can be: the groups' sizes are on the device
   const int64_t tiles = MODE == kGroupedWgrad
@@ -655,30 +655,29 @@ void launch(const GroupedArgs& a, cudaStream_t s, int slices = 1) {
   static int cache[kMaxDevices];
   if constexpr (PAIR) {
     auto kern = grouped_pair_kernel<MODE, BN, STAGES>;
-    const int n = static_cast<int>(std::min<int64_t>(std::max<int64_t>(1, tiles), resident(reinterpret_cast<const void*>(kern), L::kAlloc, true, cache)));
-    kern<<<2 * n, kThreads, L::kAlloc, s>>>(ta, tb, p);
+    const int n = static_cast<int>(std::min<int64_t>(std::max<int64_t>(1, tiles), resident(reinterpret_cast<const void*>(kern), threads_of(MODE), L::kAlloc, true, cache)));
+    kern<<<2 * n, threads_of(MODE), L::kAlloc, s>>>(ta, ta16, tb, p);
   } else {
     auto kern = grouped_kernel<MODE, BN, STAGES>;
-    const int n = static_cast<int>(std::min<int64_t>(std::max<int64_t>(1, tiles), resident(reinterpret_cast<const void*>(kern), L::kAlloc, false, cache)));
-    kern<<<n, kThreads, L::kAlloc, s>>>(ta, tb, p);
+    const int n = static_cast<int>(std::min<int64_t>(std::max<int64_t>(1, tiles), resident(reinterpret_cast<const void*>(kern), threads_of(MODE), L::kAlloc, false, cache)));
+    kern<<<n, threads_of(MODE), L::kAlloc, s>>>(ta, ta16, tb, p);
   }
   FLARE_CUDA_CHECK(cudaGetLastError());
   count_launch();
 }
 
-// The slices of the weight gradient that its output tiles leave the machine idle without: a few
-// groups of a small weight and many rows.  Each is at least 512 rows of an average group.
+// The weight gradient's tiles are 128 x 256 where N allows (515 us against 655 us for pairs on 256
+// x 256 at 131072 x 512 x 4096 in 32 groups).  A few groups of a small weight and many rows leave
+// most of the machine idle: their rows are cut into slices of at least 512 rows of an average
+// group, about a tile for each SM (33 us against 630 us for 131072 x 64 x 128 in 2 groups).
 struct WgradShape {
-  bool pair;
   int bn, slices;
 };
 WgradShape wgrad_shape(int G, int64_t R, int K, int N) {
   WgradShape w;
-  w.pair = K > 128 && N > 128;
-  w.bn = w.pair ? 256 : N > 64 ? 128 : 64;
-  const int64_t tiles = static_cast<int64_t>(G) * ceil_div(K, w.pair ? 256 : 128) * ceil_div(N, w.bn);
-  const int64_t want = w.pair ? 148 : 296, most = std::min<int64_t>(64, R / G / 512);
-  w.slices = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, want / tiles)));
+  w.bn = N > 128 ? 256 : N > 64 ? 128 : 64;
+  const int64_t tiles = static_cast<int64_t>(G) * ceil_div(K, 128) * ceil_div(N, w.bn);
+  w.slices = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(64, R / G / 512), 296 / tiles)));
   return w;
 }
 
@@ -696,18 +695,27 @@ __global__ void __launch_bounds__(256) add_slices_kernel(const float* part, int6
   }
 }
 
+// Long groups and a long contraction: pairs (423 us against 449 us for the input gradient of 131072
+// x 512 x 4096 in 32 groups).  Otherwise one CTA a tile (155 us against 177 us for 200000 x 256 x
+// 1024 in 64 groups): the widest that still gives half of the SMs one.
 template <int MODE>
 void pick(const GroupedArgs& a, cudaStream_t s) {
-  const int no = MODE == kGroupedDgrad ? a.K : a.N;
-  // rows of an average group fill a pair's 256 at least once, and both sides of the tile are used
-  if (a.R >= 256ll * a.G && no > 128) launch<MODE, true, 256, 6>(a, s);
-  else if (no > 64) launch<MODE, false, 128, 6>(a, s);
+  const int no = MODE == kGroupedDgrad ? a.K : a.N, kc = MODE == kGroupedDgrad ? a.N : a.K;
+  if (a.R >= 4096ll * a.G && kc >= 512 && no > 128) {
+    launch<MODE, true, 256, 6>(a, s);
+    return;
+  }
+  const int64_t mt = a.R / 128 + std::min<int64_t>(a.G, a.R);
+  int bn = 256;
+  while (bn > 64 && (no <= bn / 2 || mt * ceil_div(no, bn) < 74)) bn /= 2;
+  if (bn == 256) launch<MODE, false, 256, 4>(a, s);
+  else if (bn == 128) launch<MODE, false, 128, 6>(a, s);
   else launch<MODE, false, 64, 8>(a, s);
 }
 
 void wgrad(const GroupedArgs& a, cudaStream_t s) {
   const WgradShape w = wgrad_shape(a.G, a.R, a.K, a.N);
-  if (w.pair) launch<kGroupedWgrad, true, 256, 6>(a, s, w.slices);
+  if (w.bn == 256) launch<kGroupedWgrad, false, 256, 4>(a, s, w.slices);
   else if (w.bn == 128) launch<kGroupedWgrad, false, 128, 6>(a, s, w.slices);
   else launch<kGroupedWgrad, false, 64, 8>(a, s, w.slices);
   if (w.slices > 1) {
@@ -1046,7 +1054,8 @@ int64_t grouped_work_floats(int G, int64_t R, int K, int N) {
   return slices > 1 ? static_cast<int64_t>(slices) * G * K * N : 0;
 }
 
-bool grouped_few_rows(int64_t rows) { return rows <= 64; }
+// 12 us against 16 us for 16 rows of 2048 x 512 in 16 groups, 18 us against 16 us for 32.
+bool grouped_few_rows(int64_t rows) { return rows <= 16; }
 
 int64_t group_sum_work_floats(int G, int64_t R, int N) {
   return R <= kSumOneLaunch ? 0 : (ceil_div(R, sum_rows(R, ceil_div(N, 256))) + static_cast<int64_t>(G)) * N;
