@@ -22,10 +22,11 @@
 // from the tokens by a kernel of their own before the product: fetched by index
 // inside it (four rows a load), they cost 45 ns of a CTA's load unit each time,
 // 1293 us against 432 us for 131072 x 512 x 4096.
-// Variants: one CTA on 128 x 256, 128 x 128 or 128 x 64 tiles; CTA pairs on 256 x 256
-// tiles (each CTA stages half of B) for long groups.  A tile that reaches past its
-// group loads only the sixteens of rows that the group has: in a serving step that
-// is two of 128.
+// Tiles are 128 x 256, 128 x 128 or 128 x 64.  (CTA pairs on 256 x 256 tiles were no
+// faster: 554 / 446 us against 529 / 436 us for the forward product and the input
+// gradient of 131072 x 512 x 4096 in 32 groups, 177 us against 155 us for 200000 x 256
+// x 1024 in 64.)  A tile that reaches past its group loads only the sixteens of rows
+// that the group has.
 // Every sum is held in fp32 and rounded once.  Every wait is bounded.
 #include "experts.cuh"
 #include "gemm.cuh"
@@ -43,11 +44,12 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn();  // gemm_tcgen05.cu
 
 namespace {
 
+constexpr int kBM = 128;         // rows of a tile
 constexpr int kBK = 64;          // contraction step: one 128-byte swizzle atom of 16-bit values
 constexpr int kEpiWarps = 8;     // two for each quarter of the TMEM lanes, half of the columns each
 // the producer and MMA issuer warps, these, and one that zeroes the weight gradient's partial steps
 constexpr int threads_of(int mode) { return 64 + 32 * kEpiWarps + (mode == kGroupedWgrad ? 32 : 0); }
-constexpr int kTileA = 128 * kBK * 2;
+constexpr int kTileA = kBM * kBK * 2;
 
 struct GP {
   const int* offsets;
@@ -67,10 +69,9 @@ struct GP {
   uint64_t timeout_ns;
 };
 
-template <bool PAIR, int BN, int STAGES>
+template <int BN, int STAGES>
 struct Smem {
-  static constexpr int kBNh = PAIR ? BN / 2 : BN;  // B rows that one CTA stages
-  static constexpr int kTileB = kBNh * kBK * 2;
+  static constexpr int kTileB = BN * kBK * 2;
   static constexpr int kStage = kTileA + kTileB;
   static constexpr int kOffB = STAGES * kTileA;
   static constexpr int kOffEpi = kOffB + STAGES * kTileB;       // 2 KiB per epilogue warp
@@ -96,10 +97,10 @@ struct Tile {
 
 constexpr int kSortGroups = 512;
 
-// Walks this CTA's (or pair's) tiles in order.  The weight gradient's tiles differ in length: they
+// Walks this CTA's tiles in order.  The weight gradient's tiles differ in length: they
 // come by falling size of their group, dealt out back and forth, so that every CTA gets about the
 // same number of steps.
-template <int MODE, int BM, int BN>
+template <int MODE, int BN>
 struct Walk {
   const GP& p;
   const int* pre;
@@ -123,7 +124,7 @@ struct Walk {
       m -= t.slice * p.mt;
       t.g = p.G <= kSortGroups ? pre[at] : at;
       const int2 r = group_range(p, t.g);
-      t.m0 = m * BM;
+      t.m0 = m * kBM;
       const int steps = (r.y - r.x + kBK - 1) / kBK;
       const int s0 = static_cast<int>(static_cast<int64_t>(steps) * t.slice / p.slices);
       const int s1 = static_cast<int>(static_cast<int64_t>(steps) * (t.slice + 1) / p.slices);
@@ -137,7 +138,7 @@ struct Walk {
       t.g = g;
       t.lo = r.x;
       t.hi = r.y;
-      t.m0 = r.x + m * BM;
+      t.m0 = r.x + m * kBM;
       t.steps = (p.Kc + kBK - 1) / kBK;
     }
     return true;
@@ -242,13 +243,12 @@ __device__ __forceinline__ void zero_rows(uint8_t* tile, int boxes, int r) {
 }
 
 // ta / tb: tiles of A and B; ta16: A in boxes of 16 rows (forward, input gradient).
-template <int MODE, bool PAIR, int BN, int STAGES>
-__device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtensorMap& ta16, const CUtensorMap& tb,
-                                             const GP& p) {
-  using L = Smem<PAIR, BN, STAGES>;
-  constexpr int BM = PAIR ? 256 : 128;
+template <int MODE, int BN, int STAGES>
+__global__ void __launch_bounds__(threads_of(MODE), 1)
+    grouped_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap ta16,
+                   const __grid_constant__ CUtensorMap tb, const __grid_constant__ GP p) {
+  using L = Smem<BN, STAGES>;
   constexpr bool A_MN = MODE == kGroupedWgrad, B_MN = MODE != kGroupedDgrad;
-  static_assert(!(PAIR && MODE == kGroupedWgrad), "the weight gradient's tiles are one CTA's");
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* sm = smem_raw + (((raw + 1023u) & ~1023u) - raw);
@@ -260,8 +260,6 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
   uint64_t* acc_empty = acc_full + 2;
   uint32_t* slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   const int warp = warp_id(), lane = lane_id();
-  const int rank = PAIR ? static_cast<int>(sm100::cluster_ctarank()) : 0;
-  const int first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
 
   if (threadIdx.x == 0) {
     sm100::tma_prefetch_desc(&ta);
@@ -273,23 +271,18 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
     }
     for (int b = 0; b < 2; ++b) {
       sm100::mbar_init(&acc_full[b], 1);
-      sm100::mbar_init(&acc_empty[b], kEpiWarps * (PAIR ? 2 : 1));
+      sm100::mbar_init(&acc_empty[b], kEpiWarps);
     }
     sm100::fence_mbar_init();
   }
   if (warp == 0) {
-    if constexpr (PAIR) {
-      sm100::tmem_alloc_pair(slot, 2 * BN);
-      sm100::tmem_relinquish_pair();
-    } else {
-      sm100::tmem_alloc(slot, 2 * BN);
-      sm100::tmem_relinquish();
-    }
+    sm100::tmem_alloc(slot, 2 * BN);
+    sm100::tmem_relinquish();
   }
   if constexpr (MODE != kGroupedWgrad) {
     for (int g = threadIdx.x; g < p.G; g += threads_of(MODE)) {
       const int2 r = group_range(p, g);
-      pre[g + 1] = (r.y - r.x + BM - 1) / BM;
+      pre[g + 1] = (r.y - r.x + kBM - 1) / kBM;
     }
     if (threadIdx.x == 0) pre[0] = 0;
     __syncthreads();
@@ -329,26 +322,17 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
         report_error(p.status, kIndexOutOfRange, g);
   }
   sm100::tc_fence_before();
-  if constexpr (PAIR) sm100::cluster_sync();  // both CTAs' barriers and TMEM exist before any cross-CTA use
-  else __syncthreads();
+  __syncthreads();
   sm100::tc_fence_after();
   const uint32_t tmem = *slot;
   Tile t;
-  Walk<MODE, BM, BN> walk(p, pre, first, step);
+  Walk<MODE, BN> walk(p, pre, blockIdx.x, gridDim.x);
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
       uint32_t it = 0;
       bool ok = true;
-      auto load2 = [&](void* dst, const CUtensorMap& m, int s, int x, int y) {
-        if constexpr (PAIR) sm100::tma_load_2d_pair(dst, &m, sm100::mapa_shared(&full[s], 0), x, y);
-        else sm100::tma_load_2d(dst, &m, &full[s], x, y);
-      };
-      auto load3 = [&](void* dst, const CUtensorMap& m, int s, int x, int y, int z) {
-        if constexpr (PAIR) sm100::tma_load_3d_pair(dst, &m, sm100::mapa_shared(&full[s], 0), x, y, z);
-        else sm100::tma_load_3d(dst, &m, &full[s], x, y, z);
-      };
       while (ok && walk.next(t)) {
         for (int k = 0; k < t.steps; ++k, ++it) {
           const int s = it % STAGES;
@@ -358,21 +342,19 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
           }
           uint8_t* sa = sm + s * kTileA;
           uint8_t* sb = sm + L::kOffB + s * L::kTileB;
-          const int nb = t.n0 + rank * L::kBNh;
           if constexpr (MODE != kGroupedWgrad) {
-            const int k0 = k * kBK, row0 = t.m0 + rank * 128, rows = t.hi - row0;
-            if (rank == 0)
-              sm100::mbar_arrive_expect_tx(&full[s], a_bytes(rows) + L::kTileB + (PAIR ? a_bytes(rows - 128) + L::kTileB : 0));
+            const int k0 = k * kBK, rows = t.hi - t.m0;
+            sm100::mbar_arrive_expect_tx(&full[s], a_bytes(rows) + L::kTileB);
             if (rows > 64) {
-              load2(sa, ta, s, k0, row0);
+              sm100::tma_load_2d(sa, &ta, &full[s], k0, t.m0);
             } else {
-              for (int j = 0; j < a_boxes(rows); ++j) load2(sa + j * 2048, ta16, s, k0, row0 + j * 16);
+              for (int j = 0; j < a_boxes(rows); ++j) sm100::tma_load_2d(sa + j * 2048, &ta16, &full[s], k0, t.m0 + j * 16);
             }
             if constexpr (B_MN) {
 #pragma unroll
-              for (int j = 0; j < L::kBNh / 64; ++j) load3(sb + j * 8192, tb, s, nb + 64 * j, k0, t.g);
+              for (int j = 0; j < BN / 64; ++j) sm100::tma_load_3d(sb + j * 8192, &tb, &full[s], t.n0 + 64 * j, k0, t.g);
             } else {
-              load3(sb, tb, s, k0, nb, t.g);
+              sm100::tma_load_3d(sb, &tb, &full[s], k0, t.n0, t.g);
             }
           } else {
             const int r0 = t.lo + k * kBK;
@@ -381,7 +363,7 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
             sm100::tma_load_2d(sa, &ta, bar, t.m0, r0);
             sm100::tma_load_2d(sa + 8192, &ta, bar, t.m0 + 64, r0);
 #pragma unroll
-            for (int j = 0; j < L::kBNh / 64; ++j) sm100::tma_load_2d(sb + j * 8192, &tb, bar, nb + 64 * j, r0);
+            for (int j = 0; j < BN / 64; ++j) sm100::tma_load_2d(sb + j * 8192, &tb, bar, t.n0 + 64 * j, r0);
           }
         }
       }
@@ -389,10 +371,10 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
     __syncwarp();
   } else if (warp == 1) {
     // ---------------------------------------------------------- MMA issuer
-    // One thread (of the even CTA).  What it does between two steps' products is what the tensor
+    // One thread.  What it does between two steps' products is what the tensor
     // cores may wait for, so the next step's barrier is tried while this one's products are queued,
     // and descriptors are an addition each.
-    if (lane == 0 && rank == 0) {
+    if (lane == 0) {
       // 16 columns of a K-major row are 32 bytes, 16 rows of an MN-major box 2048
       constexpr int kStepA = (A_MN ? 2048 : 32) >> 4, kStepB = (B_MN ? 2048 : 32) >> 4;
       const uint64_t da0 = sm100::make_smem_desc(smem_u32(sm), A_MN ? 8192 : 16, 1024);
@@ -404,11 +386,11 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
         const int buf = i & 1;
         const uint32_t d = tmem + buf * BN;
         const int last = MODE == kGroupedWgrad ? (t.hi - t.lo) - (t.steps - 1) * kBK : kBK;  // rows of the last step
-        if (i >= 2 && !sm100::mbar_wait_cluster(&acc_empty[buf], ((i >> 1) - 1) & 1, p.timeout_ns, p.status, 420 + buf)) break;
+        if (i >= 2 && !sm100::mbar_wait(&acc_empty[buf], ((i >> 1) - 1) & 1, p.timeout_ns, p.status, 420 + buf)) break;
         sm100::tc_fence_after();
         for (int k = 0; k < t.steps; ++k) {
           const int s = it % STAGES;
-          if (!ready && !sm100::mbar_wait_cluster(&full[s], (it / STAGES) & 1, p.timeout_ns, p.status, 440 + s)) {
+          if (!ready && !sm100::mbar_wait(&full[s], (it / STAGES) & 1, p.timeout_ns, p.status, 440 + s)) {
             ok = false;
             break;
           }
@@ -418,19 +400,14 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
             for (int q = 0; q < (last + 15) / 16; ++q) sm100::mma_f16_ss(d, da + q * kStepA, db + q * kStepB, p.idesc, (k | q) != 0);
           } else {
 #pragma unroll
-            for (int q = 0; q < kBK / 16; ++q) {
-              if constexpr (PAIR) sm100::mma_f16_ss_pair(d, da + q * kStepA, db + q * kStepB, p.idesc, (k | q) != 0);
-              else sm100::mma_f16_ss(d, da + q * kStepA, db + q * kStepB, p.idesc, (k | q) != 0);
-            }
+            for (int q = 0; q < kBK / 16; ++q) sm100::mma_f16_ss(d, da + q * kStepA, db + q * kStepB, p.idesc, (k | q) != 0);
           }
-          if constexpr (PAIR) sm100::mma_commit_pair_both(&empty[s]);
-          else sm100::mma_commit(&empty[s]);
+          sm100::mma_commit(&empty[s]);
           ++it;
-          ready = sm100::mbar_test_wait_cluster(&full[it % STAGES], (it / STAGES) & 1);
+          ready = sm100::mbar_test_wait(&full[it % STAGES], (it / STAGES) & 1);
         }
         if (!ok) break;
-        if constexpr (PAIR) sm100::mma_commit_pair_both(&acc_full[buf]);
-        else sm100::mma_commit(&acc_full[buf]);
+        sm100::mma_commit(&acc_full[buf]);
         ++i;
       }
     }
@@ -448,7 +425,7 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
       if (!__all_sync(0xffffffffu, sm100::mbar_wait(&tail[s], (tails >> s) & 1, p.timeout_ns, p.status, 480 + s))) break;
       tails ^= 1u << s;
       zero_rows(sm + s * kTileA, 2, last);
-      zero_rows(sm + L::kOffB + s * L::kTileB, L::kBNh / 64, last);
+      zero_rows(sm + L::kOffB + s * L::kTileB, BN / 64, last);
       sm100::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) sm100::mbar_arrive(&full[s]);
@@ -464,7 +441,7 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
     while (walk.next(t)) {
       const int buf = i & 1;
       const bool any = t.steps > 0;
-      const int row0 = t.m0 + rank * 128 + quarter * 32;
+      const int row0 = t.m0 + quarter * 32;
       const int rows = min(32, (MODE == kGroupedWgrad ? p.Mo : t.hi) - row0);
       const int chunks = rows > 0 ? min(BN / 64, (p.No - t.n0 - c0 + 31) / 32) : 0;  // of 32 columns, with some inside
       const int64_t base = MODE == kGroupedWgrad ? (static_cast<int64_t>(t.slice) * p.G + t.g) * p.Mo * p.ldo : 0;
@@ -515,10 +492,7 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
         }
         sm100::tc_fence_before();
         __syncwarp();
-        if (lane == 0) {
-          if constexpr (PAIR) sm100::mbar_arrive_cluster(sm100::mapa_shared(&acc_empty[buf], 0));
-          else sm100::mbar_arrive(&acc_empty[buf]);
-        }
+        if (lane == 0) sm100::mbar_arrive(&acc_empty[buf]);
         ++i;
       } else if (!p.accumulate) {  // a group without rows has a gradient of zeros
         uint32_t zero[32];
@@ -530,24 +504,7 @@ __device__ __forceinline__ void grouped_body(const CUtensorMap& ta, const CUtens
   }
   sm100::tc_fence_before();
   __syncthreads();
-  if constexpr (PAIR) sm100::cluster_sync();  // neither CTA leaves while the other may signal it or read its TMEM
-  if (warp == 0) {
-    if constexpr (PAIR) sm100::tmem_dealloc_pair(tmem, 2 * BN);
-    else sm100::tmem_dealloc(tmem, 2 * BN);
-  }
-}
-
-template <int MODE, int BN, int STAGES>
-__global__ void __launch_bounds__(threads_of(MODE), 1)
-    grouped_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap ta16,
-                   const __grid_constant__ CUtensorMap tb, const __grid_constant__ GP p) {
-  grouped_body<MODE, false, BN, STAGES>(ta, ta16, tb, p);
-}
-template <int MODE, int BN, int STAGES>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads_of(MODE), 1)
-    grouped_pair_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap ta16,
-                        const __grid_constant__ CUtensorMap tb, const __grid_constant__ GP p) {
-  grouped_body<MODE, true, BN, STAGES>(ta, ta16, tb, p);
+  if (warp == 0) sm100::tmem_dealloc(tmem, 2 * BN);
 }
 
 // ------------------------------------------------------------------- host
@@ -579,41 +536,23 @@ CUtensorMap map2(const void* base, int dtype, int64_t inner, int64_t rows, int64
 
 constexpr int kMaxDevices = 64;
 
-// Sets a kernel's shared-memory limit once per device and returns how many CTAs (or pairs) of it
-// the current device runs at once.
-int resident(const void* kern, int threads, int smem, bool pair, int (&cache)[kMaxDevices]) {
+// Sets a kernel's shared-memory limit once per device; returns the current device's SMs (one CTA each).
+int prepare(const void* kern, int smem, int (&sms)[kMaxDevices]) {
   static std::mutex mu;
   int dev = 0;
   FLARE_CUDA_CHECK(cudaGetDevice(&dev));
   FLARE_CHECK(dev >= 0 && dev < kMaxDevices, "device index");
   std::lock_guard<std::mutex> lock(mu);
-  if (cache[dev] == 0) {
+  if (sms[dev] == 0) {
     FLARE_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    int n = 0;
-    if (pair) {
-      cudaLaunchConfig_t cfg{};
-      cfg.gridDim = dim3(2);
-      cfg.blockDim = dim3(threads);
-      cfg.dynamicSmemBytes = smem;
-      cudaLaunchAttribute at[1];
-      at[0].id = cudaLaunchAttributeClusterDimension;
-      at[0].val.clusterDim.x = 2;
-      at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-      cfg.attrs = at;
-      cfg.numAttrs = 1;
-      FLARE_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
-    } else {
-      FLARE_CUDA_CHECK(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
-    }
-    cache[dev] = std::max(1, n);
+    FLARE_CUDA_CHECK(cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev));
   }
-  return cache[dev];
+  return sms[dev];
 }
 
-template <int MODE, bool PAIR, int BN, int STAGES>
+template <int MODE, int BN, int STAGES>
 void launch(const GroupedArgs& a, cudaStream_t s, int slices = 1) {
-  using L = Smem<PAIR, BN, STAGES>;
-  constexpr int BM = PAIR ? 256 : 128;
+  using L = Smem<BN, STAGES>;
   GP p{};
   p.offsets = a.offsets;
   p.G = a.G;
@@ -621,7 +560,7 @@ void launch(const GroupedArgs& a, cudaStream_t s, int slices = 1) {
   p.Mo = a.K;
   p.No = MODE == kGroupedDgrad ? a.K : a.N;
   p.Kc = MODE == kGroupedDgrad ? a.N : a.K;
-  p.mt = ceil_div(a.K, BM);
+  p.mt = ceil_div(a.K, kBM);
   p.nt = ceil_div(p.No, BN);
   p.slices = slices;
   p.out = slices > 1 ? a.work : a.out;
@@ -630,7 +569,7 @@ void launch(const GroupedArgs& a, cudaStream_t s, int slices = 1) {
   p.accumulate = slices > 1 ? 0 : a.accumulate;
   p.bias = MODE == kGroupedFwd ? a.bias : nullptr;
   p.bias_dtype = a.bias_dtype;
-  p.idesc = sm100::make_idesc_16bit(BM, BN, MODE == kGroupedWgrad, MODE != kGroupedDgrad, a.dtype == kBF16);
+  p.idesc = sm100::make_idesc_16bit(kBM, BN, MODE == kGroupedWgrad, MODE != kGroupedDgrad, a.dtype == kBF16);
   p.status = a.status;
   p.timeout_ns = a.timeout_ns;
   CUtensorMap ta, ta16, tb;
@@ -640,7 +579,7 @@ void launch(const GroupedArgs& a, cudaStream_t s, int slices = 1) {
     ta16 = ta;
   } else {
     const int64_t wd[3] = {a.N, a.K, a.G}, wp[2] = {a.N, static_cast<int64_t>(a.K) * a.N};
-    const int box_fwd[3] = {64, kBK, 1}, box_bwd[3] = {64, L::kBNh, 1};
+    const int box_fwd[3] = {64, kBK, 1}, box_bwd[3] = {64, BN, 1};
     tb = make_map(a.w, a.dtype, 3, wd, wp, MODE == kGroupedFwd ? box_fwd : box_bwd);
     const void* rows = MODE == kGroupedFwd ? a.x : a.dy;
     const int64_t ld = MODE == kGroupedFwd ? a.ldx : a.lddy;
@@ -650,26 +589,19 @@ void launch(const GroupedArgs& a, cudaStream_t s, int slices = 1) {
   // as many tiles as there can be: the groups' sizes are on the device
   const int64_t tiles = MODE == kGroupedWgrad
                             ? static_cast<int64_t>(a.G) * p.mt * p.nt * slices
-                            : (a.R / BM + std::min<int64_t>(a.G, a.R)) * p.nt;
+                            : (a.R / kBM + std::min<int64_t>(a.G, a.R)) * p.nt;
   FLARE_CHECK(tiles < (1ll << 31), "grouped products: too many tiles");
-  static int cache[kMaxDevices];
-  if constexpr (PAIR) {
-    auto kern = grouped_pair_kernel<MODE, BN, STAGES>;
-    const int n = static_cast<int>(std::min<int64_t>(std::max<int64_t>(1, tiles), resident(reinterpret_cast<const void*>(kern), threads_of(MODE), L::kAlloc, true, cache)));
-    kern<<<2 * n, threads_of(MODE), L::kAlloc, s>>>(ta, ta16, tb, p);
-  } else {
-    auto kern = grouped_kernel<MODE, BN, STAGES>;
-    const int n = static_cast<int>(std::min<int64_t>(std::max<int64_t>(1, tiles), resident(reinterpret_cast<const void*>(kern), threads_of(MODE), L::kAlloc, false, cache)));
-    kern<<<n, threads_of(MODE), L::kAlloc, s>>>(ta, ta16, tb, p);
-  }
+  static int sms[kMaxDevices];
+  auto kern = grouped_kernel<MODE, BN, STAGES>;
+  const int64_t grid = std::min<int64_t>(std::max<int64_t>(1, tiles), prepare(reinterpret_cast<const void*>(kern), L::kAlloc, sms));
+  kern<<<static_cast<int>(grid), threads_of(MODE), L::kAlloc, s>>>(ta, ta16, tb, p);
   FLARE_CUDA_CHECK(cudaGetLastError());
   count_launch();
 }
 
-// The weight gradient's tiles are 128 x 256 where N allows (515 us against 655 us for pairs on 256
-// x 256 at 131072 x 512 x 4096 in 32 groups).  A few groups of a small weight and many rows leave
-// most of the machine idle: their rows are cut into slices of at least 512 rows of an average
-// group, about a tile for each SM (33 us against 630 us for 131072 x 64 x 128 in 2 groups).
+// The weight gradient's tiles are as wide as N allows.  A few groups of a small weight and many
+// rows leave most of the machine idle: their rows are cut into slices of at least 512 rows of an
+// average group, about two tiles for each SM (33 us against 630 us for 131072 x 64 x 128 in 2 groups).
 struct WgradShape {
   int bn, slices;
 };
@@ -695,29 +627,24 @@ __global__ void __launch_bounds__(256) add_slices_kernel(const float* part, int6
   }
 }
 
-// Long groups and a long contraction: pairs (423 us against 449 us for the input gradient of 131072
-// x 512 x 4096 in 32 groups).  Otherwise one CTA a tile (155 us against 177 us for 200000 x 256 x
-// 1024 in 64 groups): the widest that still gives half of the SMs one.
+// The widest tile that still gives half of the SMs one (3003 rows of 200 x 328 in 7 groups: 10.4 us
+// at 256 columns, 8.4 us at 128; 400 rows of 2048 x 512 in 8: 21 us at 256, 17 us at 64).
 template <int MODE>
 void pick(const GroupedArgs& a, cudaStream_t s) {
-  const int no = MODE == kGroupedDgrad ? a.K : a.N, kc = MODE == kGroupedDgrad ? a.N : a.K;
-  if (a.R >= 4096ll * a.G && kc >= 512 && no > 128) {
-    launch<MODE, true, 256, 6>(a, s);
-    return;
-  }
-  const int64_t mt = a.R / 128 + std::min<int64_t>(a.G, a.R);
+  const int no = MODE == kGroupedDgrad ? a.K : a.N;
+  const int64_t mt = a.R / kBM + std::min<int64_t>(a.G, a.R);
   int bn = 256;
   while (bn > 64 && (no <= bn / 2 || mt * ceil_div(no, bn) < 74)) bn /= 2;
-  if (bn == 256) launch<MODE, false, 256, 4>(a, s);
-  else if (bn == 128) launch<MODE, false, 128, 6>(a, s);
-  else launch<MODE, false, 64, 8>(a, s);
+  if (bn == 256) launch<MODE, 256, 4>(a, s);
+  else if (bn == 128) launch<MODE, 128, 6>(a, s);
+  else launch<MODE, 64, 8>(a, s);
 }
 
 void wgrad(const GroupedArgs& a, cudaStream_t s) {
   const WgradShape w = wgrad_shape(a.G, a.R, a.K, a.N);
-  if (w.bn == 256) launch<kGroupedWgrad, false, 256, 4>(a, s, w.slices);
-  else if (w.bn == 128) launch<kGroupedWgrad, false, 128, 6>(a, s, w.slices);
-  else launch<kGroupedWgrad, false, 64, 8>(a, s, w.slices);
+  if (w.bn == 256) launch<kGroupedWgrad, 256, 4>(a, s, w.slices);
+  else if (w.bn == 128) launch<kGroupedWgrad, 128, 6>(a, s, w.slices);
+  else launch<kGroupedWgrad, 64, 8>(a, s, w.slices);
   if (w.slices > 1) {
     const int64_t n = static_cast<int64_t>(a.G) * a.K * a.N;
     add_slices_kernel<<<static_cast<int>(std::min<int64_t>((n + 1023) / 1024, 148 * 8)), 256, 0, s>>>(
