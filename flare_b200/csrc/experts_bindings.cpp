@@ -2,9 +2,10 @@
 // They take tensors and allocate their outputs and scratch from the caching
 // allocator on the current stream: scratch that belongs to one call cannot be
 // shared by two captured graphs.  For a few tokens the call itself is what
-// counts, so the graph nodes are C++ (a Python node costs some 40 us a step).  Arguments are checked by
-// flare_b200/ops/experts.py; what is checked here again is what a wrong pointer
-// or size would cost.
+// counts, so the graph nodes are C++ (a Python node costs some 40 us a step) and
+// arguments are checked here (in Python the checks alone took 8 us).  The entry
+// points at the end check what a caller may get wrong; the functions above them
+// check again what a wrong pointer or size would cost.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -22,7 +23,7 @@ namespace {
 int code_of(at::ScalarType t) {
   if (t == at::kFloat) return flare::kF32;
   if (t == at::kBFloat16) return flare::kBF16;
-  TORCH_CHECK(t == at::kHalf, "expected float32, bfloat16 or float16, got ", t);
+  TORCH_CHECK(t == at::kHalf, "expected float32, bfloat16 or float16");
   return flare::kF16;
 }
 
@@ -40,7 +41,7 @@ int64_t pitch(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1);
 
 const int* ints(const Tensor& t, const Tensor& like, int64_t n, const char* what) {
   TORCH_CHECK(t.scalar_type() == at::kInt && t.is_contiguous() && t.device() == like.device() && t.numel() == n, what,
-              ": int32, contiguous, on the same device, with ", n, " values");
+              ": int32, contiguous, on the same device, with as many values as expected");
   return t.data_ptr<int>();
 }
 
@@ -49,8 +50,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> route_topk(const Tensor& logi
   TORCH_CHECK(logits.is_cuda() && logits.dim() == 3, "route_topk: logits [slots, tokens, experts] on a CUDA device");
   const c10::cuda::CUDAGuard guard(logits.device());
   const int64_t S = logits.size(0), B = logits.size(1), E = logits.size(2);
-  TORCH_CHECK(E >= 1 && E <= flare::kRouteMaxExperts, "route_topk: 1 to 512 experts, got ", E);
-  TORCH_CHECK(k >= 1 && k <= E && k <= flare::kRouteMaxTopK, "route_topk: top_k from 1 to the number of experts and 32, got ", k);
+  TORCH_CHECK(E >= 1 && E <= flare::kRouteMaxExperts, "route_topk: 1 to 512 experts");
+  TORCH_CHECK(k >= 1 && k <= E && k <= flare::kRouteMaxTopK, "route_topk: top_k from 1 to the number of experts and 32");
   TORCH_CHECK(S * E < (1ll << 31) - 1 && S * B * k < (1ll << 31) - 512, "route_topk: too many rows");
   TORCH_CHECK(E == 1 || logits.stride(2) == 1, "route_topk: logits need unit inner stride");
   Tensor experts = empty({S, B, k}, logits, at::kInt), weights = empty({S, B, k}, logits, at::kFloat);
@@ -105,7 +106,7 @@ Tensor route_topk_backward(const Tensor& experts, const Tensor& weights, const T
 
 flare::SwigluParams swiglu_params(const Tensor& x) {
   check_rows(x, "swiglu");
-  TORCH_CHECK(x.size(1) % 2 == 0, "swiglu: an even number of columns [up | gate], got ", x.size(1));
+  TORCH_CHECK(x.size(1) % 2 == 0, "swiglu: an even number of columns [up | gate]");
   flare::SwigluParams p{};
   p.x = x.data_ptr();
   p.ldx = pitch(x);
@@ -493,25 +494,72 @@ struct GroupedLinearFn : torch::autograd::Function<GroupedLinearFn> {
 };
 
 // ------------------------------------------------------------ entry points
+// Messages are put together from strings: formatting numbers through a stream here crashes (the
+// extension's and torch's C++ runtimes are not the same).
+std::string text(const char* v) { return v; }
+std::string text(int64_t v) { return std::to_string(v); }
+std::string text(at::ScalarType t) { return c10::toString(t); }
+std::string text(at::Device d) { return d.str(); }
+std::string text(at::IntArrayRef v) {
+  std::string s = "[";
+  for (size_t i = 0; i < v.size(); ++i) s += (i ? ", " : "") + std::to_string(v[i]);
+  return s + "]";
+}
+template <typename... A>
+void value_check(bool ok, const A&... what) {
+  if (!ok) throw py::value_error((text(what) + ...));
+}
+template <typename... A>
+void type_check(bool ok, const A&... what) {
+  if (!ok) throw py::type_error((text(what) + ...));
+}
+bool is_half(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf; }
+bool is_float(at::ScalarType t) { return is_half(t) || t == at::kFloat; }
+void same_device(const Tensor& a, const Tensor& b) {
+  value_check(a.device() == b.device(), "all tensors of one op must be on the same device, got ", a.device(), " and ", b.device());
+}
+
 py::tuple route_topk_op(const Tensor& logits, int64_t k) {
-  if (wants({&logits})) {
-    const auto o = RouteFn::apply(logits, k);
-    return py::make_tuple(o[0], o[1], o[2], o[3], o[4]);
+  value_check(logits.dim() == 2 || logits.dim() == 3, "logits must be [tokens, experts] or [slots, tokens, experts], got ", logits.sizes());
+  const int64_t E = logits.size(-1);
+  value_check(k >= 1 && k <= E && k <= flare::kRouteMaxTopK, "top_k must be from 1 to the number of experts (", E, ") and ",
+              flare::kRouteMaxTopK, ", got ", k);
+  value_check(E <= flare::kRouteMaxExperts, "at most ", flare::kRouteMaxExperts, " experts a slot, got ", E);
+  type_check(is_float(logits.scalar_type()), "logits must be float32, bfloat16 or float16, got ", logits.scalar_type());
+  const bool flat = logits.dim() == 2;
+  Tensor lg = flat ? logits.unsqueeze(0) : logits;
+  if (lg.stride(2) != 1 && E > 1) lg = lg.contiguous();
+  value_check(lg.size(0) * E < (1ll << 31) - 1 && lg.size(0) * lg.size(1) * k < (1ll << 31) - 512, "too many rows: 2^31 - 513 at most");
+  Tensor experts, weights, offsets, rows, row_of;
+  if (wants({&lg})) {
+    const auto o = RouteFn::apply(lg, k);
+    experts = o[0], weights = o[1], offsets = o[2], rows = o[3], row_of = o[4];
+  } else {
+    std::tie(experts, weights, offsets, rows, row_of) = route_topk(lg, k);
   }
-  const auto [experts, weights, offsets, rows, row_of] = route_topk(logits, k);
+  if (flat) experts = experts.squeeze(0), weights = weights.squeeze(0), row_of = row_of.squeeze(0);
   return py::make_tuple(experts, weights, offsets, rows, row_of);
 }
 
 Tensor swiglu_op(const Tensor& x, bool keep) {
+  value_check(x.dim() == 2 && x.size(1) % 2 == 0, "x must be [rows, 2h], got ", x.sizes());
+  type_check(is_float(x.scalar_type()), "x must be float32, bfloat16 or float16, got ", x.scalar_type());
   const Tensor v = unit_rows(x);
   if (wants({&v})) return SwigluFn::apply(v, keep);
   return std::get<0>(swiglu_forward(v, false));
 }
 
 Tensor combine_rows_op(const Tensor& z, const optional<Tensor>& weights, const Tensor& offsets, const Tensor& row_of) {
+  value_check(z.dim() == 2 && z.size(0) == row_of.numel() && row_of.dim() >= 2, "z must be [", row_of.numel(), ", n] for this route, got ", z.sizes());
+  type_check(is_float(z.scalar_type()), "z must be float32, bfloat16 or float16, got ", z.scalar_type());
+  same_device(z, row_of);
   const Tensor v = unit_rows(z);
   optional<Tensor> w;
-  if (weights.has_value()) w = weights->to(at::kFloat).contiguous();
+  if (weights.has_value()) {
+    value_check(weights->numel() == row_of.numel(), "weights must have the shape ", row_of.sizes(), ", got ", weights->sizes());
+    same_device(z, *weights);
+    w = weights->to(at::kFloat).contiguous();
+  }
   if (wants({&v}) || (w.has_value() && wants({&*w}))) return CombineFn::apply(v, w, offsets, row_of);
   const int64_t k = row_of.size(-1);
   return combine_forward(v, row_of, w, row_of.numel() / k, k, v.scalar_type());
@@ -520,10 +568,34 @@ Tensor combine_rows_op(const Tensor& z, const optional<Tensor>& weights, const T
 Tensor grouped_linear_op(const Tensor& x, const Tensor& weight, const optional<Tensor>& bias, const Tensor& offsets, const optional<Tensor>& rows,
                          const optional<Tensor>& row_of, const optional<Tensor>& flat_w, const optional<Tensor>& flat_b, int64_t status,
                          int64_t timeout_ns) {
+  value_check(x.dim() == 2 && weight.dim() >= 3 && weight.size(-2) == x.size(1), "x must be [rows, in] and weight [.., in, out], got ", x.sizes(),
+              " and ", weight.sizes());
+  const int64_t K = weight.size(-2), N = weight.size(-1);
+  type_check(is_half(x.scalar_type()) && (weight.scalar_type() == x.scalar_type() || weight.scalar_type() == at::kFloat),
+             "x must be bfloat16 or float16 and weight of the same type or float32, got ", x.scalar_type(), " and ", weight.scalar_type());
+  value_check(K > 0 && N > 0 && K % 8 == 0 && N % 8 == 0, "in and out must be multiples of 8, got ", K, " and ", N);
+  const int64_t groups = weight.numel() / (K * N);
+  value_check(groups >= 1 && groups <= flare::kGroupedMaxGroups, "1 to ", flare::kGroupedMaxGroups, " groups, got ", groups);
+  same_device(x, weight);
+  same_device(x, offsets);
+  value_check(offsets.scalar_type() == at::kInt && offsets.dim() == 1 && offsets.size(0) == groups + 1 && offsets.is_contiguous(), "offsets must be int32 [",
+              groups + 1, "] for ", groups, " groups, got ", offsets.scalar_type(), " ", offsets.sizes());
+  if (rows.has_value()) {
+    value_check(row_of.has_value() && row_of->dim() >= 1 && row_of->numel() == rows->numel() && row_of->numel() == x.size(0) * row_of->size(-1), "route of ",
+                rows->numel(), " rows does not fit ", x.size(0), " tokens");
+    same_device(x, *rows);
+    same_device(x, *row_of);
+  }
+  value_check((rows.has_value() ? rows->numel() : x.size(0)) < (1ll << 31) - 512, "too many rows: 2^31 - 513 at most");
+  if (bias.has_value()) {
+    value_check(bias->dim() >= 1 && bias->size(-1) == N && bias->numel() == groups * N, "bias must be [.., ", N, "] for ", groups, " groups, got ", bias->sizes());
+    type_check(is_float(bias->scalar_type()), "bias must be float32, bfloat16 or float16, got ", bias->scalar_type());
+    same_device(x, *bias);
+  }
   const Tensor v = tma_rows(x);
   optional<Tensor> b;
   if (bias.has_value()) b = bias->contiguous();
-  Tensor w = weight.detach().reshape({-1, weight.size(-2), weight.size(-1)}).to(x.scalar_type()).contiguous();
+  Tensor w = weight.detach().reshape({groups, K, N}).to(x.scalar_type()).contiguous();
   if (reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 != 0) w = w.clone();
   if (wants({&v, &weight}) || (b.has_value() && wants({&*b})))
     return GroupedLinearFn::apply(v, weight, b, offsets, row_of, flat_w, flat_b, w, status, timeout_ns);

@@ -37,8 +37,17 @@ MAX_TOP_K = 32
 MAX_GROUPS = 2048   # of one grouped product
 GROUP = 32          # columns that share one power-of-two scale of the 8-bit checkpoint
 
-_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
-_HALVES = (torch.bfloat16, torch.float16)
+
+
+_STATUS: dict[int, int] = {}
+
+
+def _status(x: torch.Tensor) -> int:
+    """Address of the status word of x's device (looked up once a device: a serving step pays for every call)."""
+    at = _STATUS.get(x.get_device())
+    if at is None:
+        at = _STATUS[x.get_device()] = default_status(x.device).ptr
+    return at
 
 
 class ExpertRoute(NamedTuple):
@@ -85,23 +94,13 @@ def route_topk(logits: torch.Tensor, top_k: int) -> ExpertRoute:
     ``weights`` is the softmax over the chosen logits in float32 and is differentiable; the gradient of a logit
     that was not chosen is zero.
     """
+    if logits.is_cuda:
+        return ExpertRoute(*native().route_topk(logits, top_k))
     if logits.dim() not in (2, 3):
         raise ValueError(f"logits must be [tokens, experts] or [slots, tokens, experts], got {tuple(logits.shape)}")
     if not 1 <= top_k <= min(logits.shape[-1], MAX_TOP_K):
         raise ValueError(f"top_k must be from 1 to the number of experts ({logits.shape[-1]}) and {MAX_TOP_K}, got {top_k}")
-    if not logits.is_cuda:
-        return route_topk_reference(logits, top_k)
-    if logits.dtype not in _FLOATS:
-        raise TypeError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
-    if logits.shape[-1] > MAX_EXPERTS:
-        raise ValueError(f"at most {MAX_EXPERTS} experts a slot, got {logits.shape[-1]}")
-    lg = logits if logits.dim() == 3 else logits.unsqueeze(0)
-    if lg.stride(2) != 1:
-        lg = lg.contiguous()
-    out = native().route_topk(lg, top_k)
-    if logits.dim() == 2:
-        out = (out[0][0], out[1][0], out[2], out[3], out[4][0])
-    return ExpertRoute(*out)
+    return route_topk_reference(logits, top_k)
 
 
 # ------------------------------------------------------------ grouped products
@@ -129,12 +128,6 @@ def grouped_linear_reference(x, weight, bias=None, *, offsets, rows=None):
     return torch.cat(parts)
 
 
-def _flat_grad(p: torch.Tensor | None) -> torch.Tensor | None:
-    """The fp32 view of the flat gradient buffer that a fused optimizer bound to this parameter: its gradient is
-    added there by the kernel, as for the layers of ``models.layers``."""
-    return getattr(p, "_flare_grad", None) if p is not None else None
-
-
 def grouped_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
                    offsets: torch.Tensor | None = None, route: ExpertRoute | None = None) -> torch.Tensor:
     """Every row times its group's weight: ``y[r] = x[r] @ weight[g] + bias[g]`` for the rows of group ``g``.
@@ -146,33 +139,28 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
     bfloat16 or float16, and ``in`` and ``out`` are multiples of 8.  Returns ``[R, out]``; a row of no group is zero.
     Offsets that fall, or leave ``0 .. R``, are clamped and reported by ``default_status(device).check()``.
     """
+    rows = row_of = None
     if (offsets is None) == (route is None):
         raise ValueError("give exactly one of route and offsets")
+    if route is not None:
+        offsets, rows, row_of = route.offsets, route.rows, route.row_of
+    if x.is_cuda:
+        # a parameter bound to a flat fused optimizer (``_flare_grad``: its fp32 view of the gradient buffer) gets its
+        # gradient added there by the kernel, as in the layers of ``models.layers``
+        return native().grouped_linear(x, weight, bias, offsets, rows, row_of, getattr(weight, "_flare_grad", None),
+                                       getattr(bias, "_flare_grad", None), _status(x), DEFAULT_TIMEOUT_NS)
+    on_cuda(x, weight, offsets, *(t for t in (bias, rows) if t is not None))  # refuses a mixture of devices
     if x.dim() != 2 or weight.dim() < 3 or weight.shape[-2] != x.shape[1]:
         raise ValueError(f"x must be [rows, in] and weight [.., in, out], got {tuple(x.shape)} and {tuple(weight.shape)}")
     K, N = weight.shape[-2:]
     groups = weight.numel() // max(K * N, 1)
-    rows = row_of = None
-    if route is not None:
-        offsets, rows, row_of = route.offsets, route.rows, route.row_of
-        if row_of.numel() != rows.numel() or row_of.numel() != x.shape[0] * row_of.shape[-1]:
-            raise ValueError(f"route of {rows.numel()} rows does not fit {x.shape[0]} tokens")
+    if route is not None and (row_of.numel() != rows.numel() or row_of.numel() != x.shape[0] * row_of.shape[-1]):
+        raise ValueError(f"route of {rows.numel()} rows does not fit {x.shape[0]} tokens")
     if offsets.dtype != torch.int32 or offsets.shape != (groups + 1,):
         raise ValueError(f"offsets must be int32 [{groups + 1}] for {groups} groups, got {offsets.dtype} {tuple(offsets.shape)}")
     if bias is not None and (bias.shape[-1] != N or bias.numel() != groups * N):
         raise ValueError(f"bias must be [.., {N}] for {groups} groups, got {tuple(bias.shape)}")
-    if not on_cuda(x, weight, offsets, *(t for t in (bias, rows) if t is not None)):
-        return grouped_linear_reference(x, weight, bias, offsets=offsets, rows=rows)
-    if x.dtype not in _HALVES or weight.dtype not in (x.dtype, torch.float32):
-        raise TypeError(f"x must be bfloat16 or float16 and weight of the same type or float32, got {x.dtype} and {weight.dtype}")
-    if bias is not None and bias.dtype not in _FLOATS:
-        raise TypeError(f"bias must be float32, bfloat16 or float16, got {bias.dtype}")
-    if K == 0 or N == 0 or K % 8 or N % 8:
-        raise ValueError(f"in and out must be multiples of 8, got {K} and {N}")
-    if not 1 <= groups <= MAX_GROUPS:
-        raise ValueError(f"1 to {MAX_GROUPS} groups, got {groups}")
-    return native().grouped_linear(x, weight, bias, offsets, rows, row_of, _flat_grad(weight), _flat_grad(bias),
-                                   default_status(x.device).ptr, DEFAULT_TIMEOUT_NS)
+    return grouped_linear_reference(x, weight, bias, offsets=offsets, rows=rows)
 
 
 # -------------------------------------------------------------------- SwiGLU
@@ -230,12 +218,10 @@ def swiglu(x: torch.Tensor, *, checkpoint: str | None = None) -> torch.Tensor:
     """
     if checkpoint not in (None, "e4m3"):
         raise ValueError(f"checkpoint must be None or 'e4m3', got {checkpoint!r}")
+    if x.is_cuda:
+        return native().swiglu(x, checkpoint is not None)
     if x.dim() != 2 or x.shape[1] % 2:
         raise ValueError(f"x must be [rows, 2h], got {tuple(x.shape)}")
-    if x.is_cuda:
-        if x.dtype not in _FLOATS:
-            raise TypeError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
-        return native().swiglu(x, checkpoint is not None)
     return _SwigluPlainFn.apply(x, checkpoint is not None)
 
 
@@ -259,15 +245,14 @@ def combine_rows(z: torch.Tensor, route: ExpertRoute, weights: torch.Tensor | No
     ``weights`` (``route.weights``, or any of its shape) may be left out for the plain sum.  Sums are in float32, in
     order of ``j``; a token without rows gets zeros.
     """
-    if z.dim() != 2 or z.shape[0] != route.rows.numel():
-        raise ValueError(f"z must be [{route.rows.numel()}, n] for this route, got {tuple(z.shape)}")
+    if z.is_cuda:
+        return native().combine_rows(z, weights, route.offsets, route.row_of)
+    if z.dim() != 2 or z.shape[0] != route.row_of.numel():
+        raise ValueError(f"z must be [{route.row_of.numel()}, n] for this route, got {tuple(z.shape)}")
     if weights is not None and weights.numel() != route.row_of.numel():
         raise ValueError(f"weights must have the shape {tuple(route.row_of.shape)}, got {tuple(weights.shape)}")
-    if not on_cuda(z, route.row_of, *(() if weights is None else (weights,))):
-        return combine_rows_reference(z, route, weights)
-    if z.dtype not in _FLOATS:
-        raise TypeError(f"z must be float32, bfloat16 or float16, got {z.dtype}")
-    return native().combine_rows(z, weights, route.offsets, route.row_of)
+    on_cuda(z, route.row_of, *(() if weights is None else (weights,)))  # refuses a mixture of devices
+    return combine_rows_reference(z, route, weights)
 
 
 # ------------------------------------------------------------ the whole block

@@ -221,3 +221,35 @@ def test_refusals():
     with pytest.raises(ValueError, match="routed"):
         BatchedExpertMoE(1, 4, 2, 3, True, 2, checkpoint="e4m3")
     assert ExpertRoute._fields == ("experts", "weights", "offsets", "rows", "row_of")
+
+
+def test_native_refusals():
+    """The native entry points check their arguments before they touch a device."""
+    from flare_b200._native import available, native
+
+    if not available():
+        pytest.skip("the native extension is not built")
+    C = native()
+    x, w, off = torch.zeros(4, 16).bfloat16(), torch.zeros(3, 16, 24).bfloat16(), torch.zeros(4, dtype=torch.int32)
+
+    def linear(x=x, w=w, bias=None, off=off, rows=None, row_of=None):
+        return C.grouped_linear(x, w, bias, off, rows, row_of, None, None, 0, 0)
+
+    row_of = torch.zeros(4, 2, dtype=torch.int32)
+    for call, kind, words in (
+            (lambda: linear(x=x[0]), ValueError, r"got \[16\]"), (lambda: linear(w=w[:, :8]), ValueError, r"\[3, 8, 24\]"),
+            (lambda: linear(x=x.float()), TypeError, "got Float"), (lambda: linear(w=w.half()), TypeError, "Half"),
+            (lambda: linear(w=w[:, :, :20]), ValueError, "got 16 and 20"), (lambda: linear(off=off[:2]), ValueError, "for 3 groups"),
+            (lambda: linear(off=off.long()), ValueError, "int32"), (lambda: linear(bias=w[0]), ValueError, "bias"),
+            (lambda: linear(bias=torch.zeros(3, 24).double()), TypeError, "bias"),
+            (lambda: linear(rows=off, row_of=row_of), ValueError, "does not fit 4 tokens"),
+            (lambda: linear(w=torch.zeros(2049, 16, 8).bfloat16()), ValueError, "groups, got 2049"),
+            (lambda: C.route_topk(x[0], 1), ValueError, "logits"), (lambda: C.route_topk(x, 17), ValueError, "got 17"),
+            (lambda: C.route_topk(torch.zeros(2, 513), 1), ValueError, "got 513"), (lambda: C.route_topk(x.double(), 1), TypeError, "Double"),
+            (lambda: C.swiglu(x[:, :5], False), ValueError, r"got \[4, 5\]"), (lambda: C.swiglu(x.double(), False), TypeError, "Double"),
+            (lambda: C.combine_rows(x, None, off, row_of), ValueError, r"must be \[8, n\]"),
+            (lambda: C.combine_rows(torch.zeros(8, 3), torch.zeros(7), off, row_of), ValueError, "weights"),
+            (lambda: C.combine_rows(torch.zeros(8, 3).double(), None, off, row_of), TypeError, "Double"),
+            (lambda: linear(), RuntimeError, "CUDA device")):
+        with pytest.raises(kind, match=words):
+            call()
