@@ -7,6 +7,7 @@ namespace flare {
 
 constexpr int kRouteMaxExperts = 512;  // per slot
 constexpr int kRouteMaxTopK = 32;
+constexpr int kRouteMaxGroups = 65536;  // every block of the last pass reads all groups' sizes
 
 struct RouteParams {
   const void* logits;  // [S][B][E], inner stride 1

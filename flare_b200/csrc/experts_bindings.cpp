@@ -529,7 +529,8 @@ py::tuple route_topk_op(const Tensor& logits, int64_t k) {
   const bool flat = logits.dim() == 2;
   Tensor lg = flat ? logits.unsqueeze(0) : logits;
   if (lg.stride(2) != 1 && E > 1) lg = lg.contiguous();
-  value_check(lg.size(0) * E < (1ll << 31) - 1 && lg.size(0) * lg.size(1) * k < (1ll << 31) - 512, "too many rows: 2^31 - 513 at most");
+  value_check(lg.size(0) * E <= flare::kRouteMaxGroups, "at most ", flare::kRouteMaxGroups, " groups (slots * experts), got ", lg.size(0) * E);
+  value_check(lg.size(0) * lg.size(1) * k < (1ll << 31) - 512, "too many rows: 2^31 - 513 at most");
   Tensor experts, weights, offsets, rows, row_of;
   if (wants({&lg})) {
     const auto o = RouteFn::apply(lg, k);

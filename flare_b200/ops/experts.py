@@ -34,10 +34,9 @@ from .._native import DEFAULT_TIMEOUT_NS, default_status, native, on_cuda
 
 MAX_EXPERTS = 512   # of one slot
 MAX_TOP_K = 32
+MAX_ROUTE_GROUPS = 65536  # slots * experts of one route
 MAX_GROUPS = 2048   # of one grouped product
 GROUP = 32          # columns that share one power-of-two scale of the 8-bit checkpoint
-
-
 
 _STATUS: dict[int, int] = {}
 
@@ -135,9 +134,12 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
     Exactly one of ``route`` and ``offsets`` is given.  With ``route`` the rows are gathered, ``x`` is ``[tokens,
     in]`` and row ``r`` is token ``route.rows[r]``; with ``offsets`` (int32 ``[groups + 1]``, on the device) ``x`` is
     ``[R, in]`` in group order.  ``weight`` is ``[.., in, out]`` with ``groups`` matrices in all, ``bias`` ``[.., out]``;
-    they may be float32 (they are rounded to x's type, and their gradients come back in float32).  On CUDA ``x`` is
-    bfloat16 or float16, and ``in`` and ``out`` are multiples of 8.  Returns ``[R, out]``; a row of no group is zero.
-    Offsets that fall, or leave ``0 .. R``, are clamped and reported by ``default_status(device).check()``.
+    they may be float32 (the weight is rounded to x's type; gradients come back in the types of the operands).  On CUDA
+    ``x`` is bfloat16 or float16, and ``in`` and ``out`` are multiples of 8.  Returns ``[R, out]``; a row of no group is
+    zero.  Offsets that fall, or leave ``0 .. R``, are clamped and reported by ``default_status(device).check()``.
+
+    Sums are in float32 and rounded once.  For the backward pass the gathered rows and the rounded weight are kept; a
+    token's input gradient is summed over its rows in float32.
     """
     rows = row_of = None
     if (offsets is None) == (route is None):

@@ -107,6 +107,8 @@ SIZES = {
     "past a tile": [129, 127, 257],
     "large": [700, 1, 900, 0, 333],
     "many small": [(i * 7) % 5 for i in range(300)],
+    "more than are sorted": [(i * 5) % 4 for i in range(600)],
+    "long, sums in chunks": [1, 4095, 0, 5000, 32, 100, 0],
 }
 
 
@@ -255,6 +257,40 @@ def test_grouped_linear_bad_offsets_are_reported(cuda):
         grouped_linear(x, w, offsets=torch.tensor(off, dtype=torch.int32, device=cuda))
         with pytest.raises(RuntimeError, match="out of range"):
             st.check("offsets")
+
+
+@pytest.mark.parametrize("R,G", [(9000, 1), (5000, 3)])
+def test_grouped_linear_in_slices(cuda, R, G):
+    """Few groups of a small weight: the weight gradient's rows are cut into slices, written and accumulated."""
+    gen = torch.Generator(device="cuda").manual_seed(R)
+    sizes = [R] if G == 1 else [R - 70, 0, 70]
+    off = offsets_of(sizes, 0, cuda)
+    x, dy = torch.randn(R, 40, device=cuda, generator=gen).to(BF16), torch.randn(R, 72, device=cuda, generator=gen).to(BF16)
+    w = torch.randn(G, 40, 72, device=cuda, generator=gen).to(BF16).requires_grad_(True)
+    b = torch.randn(G, 72, device=cuda, generator=gen).requires_grad_(True)
+    y = grouped_linear(x, w, b, offsets=off)
+    dw, db = torch.autograd.grad(y, (w, b), dy)
+    _, _, (dw0, aw), (db0, ab) = exact_linear(x, w.detach(), b.detach(), off, dy)
+    within(dw, dw0, (R + 2) * 2 ** -23 * aw, "dw")
+    within(db, db0, (R + 2) * 2 ** -23 * ab, "db")
+    p = torch.nn.Parameter(w.detach())
+    p._flare_grad = torch.ones_like(p, dtype=FP32)
+    grouped_linear(x, p, offsets=off).backward(dy)
+    within(p._flare_grad, 1 + dw0, (R + 3) * 2 ** -23 * (1 + aw), "accumulated")
+
+
+def test_grouped_linear_frozen_operands(cuda):
+    """Only what requires a gradient gets one: the bias alone, the input alone, the weight alone."""
+    route = route_topk(torch.randn(300, 4, device=cuda), 2)
+    x, dy = torch.randn(300, 32, device=cuda).to(BF16), torch.randn(600, 48, device=cuda).to(BF16)
+    w, b = torch.randn(4, 32, 48, device=cuda).to(BF16), torch.randn(4, 48, device=cuda).to(BF16)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    want = torch.autograd.grad(grouped_linear(*leaves, route=route), leaves, dy)
+    for i in range(3):
+        args = [x, w, b]
+        args[i] = args[i].clone().requires_grad_(True)
+        got, = torch.autograd.grad(grouped_linear(*args, route=route), args[i], dy)
+        assert torch.equal(got, want[i])
 
 
 def test_grouped_linear_flat_gradients(cuda):
@@ -594,6 +630,8 @@ def test_refusals(cuda):
         route_topk(torch.randn(2, MAX_EXPERTS + 1, device=cuda), 2)
     with pytest.raises(ValueError, match="top_k"):
         route_topk(torch.randn(2, 64, device=cuda), 33)
+    with pytest.raises(ValueError, match="groups"):
+        route_topk(torch.empty(8193, 0, 8, device=cuda), 2)
     with pytest.raises(TypeError, match="float32"):
         route_topk(lg.double(), 2)
     with pytest.raises(TypeError, match="float32"):
