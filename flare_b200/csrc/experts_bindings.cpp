@@ -299,8 +299,8 @@ void grouped_weight_grad(const Tensor& x, const Tensor& dy, const Tensor& offset
   TORCH_CHECK(x.scalar_type() == dy.scalar_type() && x.device() == dy.device() && x.size(0) == dy.size(0),
               "grouped_linear: gradient of another type or size");
   TORCH_CHECK(dw.is_contiguous() && dw.device() == x.device() && dw.numel() == G * x.size(1) * dy.size(1) &&
-                  (!accumulate || dw.scalar_type() == at::kFloat),
-              "grouped_linear: weight gradient [groups, in, out], accumulated in float32");
+                  reinterpret_cast<uintptr_t>(dw.data_ptr()) % 16 == 0 && (!accumulate || dw.scalar_type() == at::kFloat),
+              "grouped_linear: weight gradient [groups, in, out], 16-byte aligned, accumulated in float32");
   flare::GroupedArgs a{};
   a.mode = flare::kGroupedWgrad;
   a.dtype = code_of(x.scalar_type());
