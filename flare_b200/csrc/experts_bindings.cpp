@@ -217,6 +217,7 @@ std::tuple<Tensor, optional<Tensor>> combine_backward(const optional<Tensor>& z,
     p.weights = weights->data_ptr<float>();
     dw = empty({T * k}, dy, at::kFloat);
     p.dw = dw->data_ptr<float>();
+    if (N == 0) dw->zero_();
   }
   flare::combine_backward(p, stream());
   return {dz, dw};
@@ -551,7 +552,8 @@ Tensor swiglu_op(const Tensor& x, bool keep) {
 }
 
 Tensor combine_rows_op(const Tensor& z, const optional<Tensor>& weights, const Tensor& offsets, const Tensor& row_of) {
-  value_check(z.dim() == 2 && z.size(0) == row_of.numel() && row_of.dim() >= 2, "z must be [", row_of.numel(), ", n] for this route, got ", z.sizes());
+  value_check(row_of.dim() >= 2 && row_of.size(-1) >= 1, "row_of must be [.., tokens, choices], got ", row_of.sizes());
+  value_check(z.dim() == 2 && z.size(0) == row_of.numel(), "z must be [", row_of.numel(), ", n] for this route, got ", z.sizes());
   type_check(is_float(z.scalar_type()), "z must be float32, bfloat16 or float16, got ", z.scalar_type());
   same_device(z, row_of);
   const Tensor v = unit_rows(z);
@@ -582,7 +584,7 @@ Tensor grouped_linear_op(const Tensor& x, const Tensor& weight, const optional<T
   value_check(offsets.scalar_type() == at::kInt && offsets.dim() == 1 && offsets.size(0) == groups + 1 && offsets.is_contiguous(), "offsets must be int32 [",
               groups + 1, "] for ", groups, " groups, got ", offsets.scalar_type(), " ", offsets.sizes());
   if (rows.has_value()) {
-    value_check(row_of.has_value() && row_of->dim() >= 1 && row_of->numel() == rows->numel() && row_of->numel() == x.size(0) * row_of->size(-1), "route of ",
+    value_check(row_of.has_value() && row_of->dim() >= 1 && row_of->size(-1) >= 1 && row_of->numel() == rows->numel() && row_of->numel() == x.size(0) * row_of->size(-1), "route of ",
                 rows->numel(), " rows does not fit ", x.size(0), " tokens");
     same_device(x, *rows);
     same_device(x, *row_of);

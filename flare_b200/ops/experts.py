@@ -30,6 +30,7 @@ from typing import NamedTuple
 import torch
 from torch.autograd.function import once_differentiable
 
+from .. import _native
 from .._native import DEFAULT_TIMEOUT_NS, default_status, native, on_cuda
 
 MAX_EXPERTS = 512   # of one slot
@@ -42,9 +43,12 @@ _STATUS: dict[int, int] = {}
 
 
 def _status(x: torch.Tensor) -> int:
-    """Address of the status word of x's device (looked up once a device: a serving step pays for every call)."""
+    """Address of the status word of x's device (looked up once a device: a serving step pays for every call).  The word
+    is not made inside a capture: its zeros would be part of the graph, and nothing would clear it before a replay."""
     at = _STATUS.get(x.get_device())
     if at is None:
+        if x.get_device() not in _native._STATUS and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the first call on a device cannot be captured into a CUDA graph: make one before the capture")
         at = _STATUS[x.get_device()] = default_status(x.device).ptr
     return at
 

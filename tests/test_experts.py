@@ -248,8 +248,22 @@ def test_native_refusals():
             (lambda: C.route_topk(torch.zeros(2, 513), 1), ValueError, "got 513"), (lambda: C.route_topk(x.double(), 1), TypeError, "Double"),
             (lambda: C.swiglu(x[:, :5], False), ValueError, r"got \[4, 5\]"), (lambda: C.swiglu(x.double(), False), TypeError, "Double"),
             (lambda: C.combine_rows(x, None, off, row_of), ValueError, r"must be \[8, n\]"),
+            (lambda: C.combine_rows(x[:0], None, off, row_of[:, :0]), ValueError, "choices"),
+            (lambda: linear(rows=off[:0], row_of=row_of[:, :0]), ValueError, "does not fit"),
             (lambda: C.combine_rows(torch.zeros(8, 3), torch.zeros(7), off, row_of), ValueError, "weights"),
             (lambda: C.combine_rows(torch.zeros(8, 3).double(), None, off, row_of), TypeError, "Double"),
             (lambda: linear(), RuntimeError, "CUDA device")):
         with pytest.raises(kind, match=words):
             call()
+
+
+def test_first_call_in_a_capture_is_refused(monkeypatch):
+    from flare_b200 import _native
+    from flare_b200.ops import experts
+
+    monkeypatch.setattr(experts, "_STATUS", {})
+    monkeypatch.setattr(_native, "_STATUS", {})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="before the capture"):
+        experts._status(torch.zeros(1))
+    assert not experts._STATUS and not _native._STATUS

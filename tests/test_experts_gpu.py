@@ -602,6 +602,9 @@ def test_no_rows(cuda):
     assert not y.any() and not out.any()
     gx, gw, gb = torch.autograd.grad(out, (x, w, b), torch.ones_like(out))
     assert not gx.any() and not gw.any() and not gb.any()
+    z, v = torch.empty(10, 0, device=cuda, requires_grad=True), torch.ones(5, 2, device=cuda, requires_grad=True)
+    gz, gv = torch.autograd.grad(combine_rows(z, route, v), (z, v), torch.empty(5, 0, device=cuda))  # rows of no columns
+    assert gz.shape == z.shape and not gv.any()
     for checkpoint in (None, "e4m3"):
         h = torch.empty(0, 8, device=cuda, dtype=BF16, requires_grad=True)
         assert torch.autograd.grad(swiglu(h, checkpoint=checkpoint), h, torch.empty(0, 4, device=cuda, dtype=BF16))[0].shape == (0, 8)
