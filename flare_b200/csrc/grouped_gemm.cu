@@ -90,9 +90,22 @@ struct Smem {
   static_assert(kAlloc <= 227 * 1024, "shared memory of one CTA");
 };
 
-__device__ __forceinline__ int2 group_range(const GP& p, int g) {
-  const int lo = min(max(p.offsets[g], 0), p.R);
-  return make_int2(lo, min(max(p.offsets[g + 1], lo), p.R));
+// Rows of group g: offsets are clamped to the rows, and a group starts at the largest offset up to
+// its own, so that no two groups share a row whatever the offsets are (a row that two had would be
+// written by two CTAs).  Where the offsets rise, that is its own offset: `falls` says that they do not.
+__device__ __forceinline__ int clamped(const GP& p, int g) { return min(max(p.offsets[g], 0), p.R); }
+__device__ __forceinline__ int2 group_range(const GP& p, int g, bool falls) {
+  int lo = clamped(p, g);
+  if (falls)
+    for (int o = 0; o < g; ++o) lo = max(lo, clamped(p, o));
+  return make_int2(lo, max(lo, clamped(p, g + 1)));
+}
+// The same by a whole warp, which needs no flag (32 offsets at a time).
+__device__ __forceinline__ int2 group_range_warp(const GP& p, int g) {
+  int lo = 0;
+  for (int o = lane_id(); o <= g; o += 32) lo = max(lo, clamped(p, o));
+  lo = __reduce_max_sync(0xffffffffu, lo);
+  return make_int2(lo, max(lo, clamped(p, g + 1)));
 }
 
 struct Tile {
@@ -111,9 +124,10 @@ struct Walk {
   const GP& p;
   const int* pre;
   int turn, me, step, total, g;
-  __device__ Walk(const GP& p_, const int* pre_, int first, int step_)
+  bool falls;
+  __device__ Walk(const GP& p_, const int* pre_, int first, int step_, bool falls_)
       : p(p_), pre(pre_), turn(0), me(first), step(step_),
-        total(MODE == kGroupedWgrad ? p_.G * p_.mt * p_.nt * p_.slices : pre_[p_.G] * p_.nt), g(0) {}
+        total(MODE == kGroupedWgrad ? p_.G * p_.mt * p_.nt * p_.slices : pre_[p_.G] * p_.nt), g(0), falls(falls_) {}
   __device__ bool next(Tile& t) {
     int u = turn * step + me;
     if (MODE == kGroupedWgrad && (turn & 1)) u = turn * step + (step - 1 - me);
@@ -129,7 +143,7 @@ struct Walk {
       t.slice = m / p.mt;
       m -= t.slice * p.mt;
       t.g = p.G <= kSortGroups ? pre[at] : at;
-      const int2 r = group_range(p, t.g);
+      const int2 r = group_range(p, t.g, falls);
       t.m0 = m * kBM;
       const int steps = (r.y - r.x + kBK - 1) / kBK;
       const int s0 = static_cast<int>(static_cast<int64_t>(steps) * t.slice / p.slices);
@@ -140,7 +154,7 @@ struct Walk {
     } else {
       while (pre[g + 1] <= m) ++g;
       m -= pre[g];
-      const int2 r = group_range(p, g);
+      const int2 r = group_range(p, g, falls);
       t.g = g;
       t.lo = r.x;
       t.hi = r.y;
@@ -227,9 +241,9 @@ __device__ __forceinline__ void regs_ready(uint32_t (&r)[32]) {
 }
 
 // Rows outside every group (before the first, behind the last) become zeros.
-__device__ __forceinline__ void zero_outside(const GP& p, int warp, int warps) {
+__device__ __forceinline__ void zero_outside(const GP& p, int warp, int warps, bool falls) {
   const int lane = lane_id();
-  const int first = group_range(p, 0).x, last = group_range(p, p.G - 1).y;
+  const int first = clamped(p, 0), last = group_range(p, p.G - 1, falls).y;
   const int64_t n = static_cast<int64_t>(first) + (p.R - last);
   for (int64_t i = warp; i < n; i += warps) {
     const int64_t r = i < first ? i : last + (i - first);
@@ -285,13 +299,30 @@ __global__ void __launch_bounds__(threads_of(MODE), 1)
     sm100::tmem_alloc(slot, 2 * BN);
     sm100::tmem_relinquish();
   }
-  if constexpr (MODE != kGroupedWgrad) {
+  // A group that ends before it starts, or outside the rows, is reported by the first CTA; every one
+  // has to know of those that fall.  pre: tiles of the groups, or (weight gradient) their sizes.
+  constexpr bool kWgrad = MODE == kGroupedWgrad;
+  auto sizes = [&](bool f) {
     for (int g = threadIdx.x; g < p.G; g += threads_of(MODE)) {
-      const int2 r = group_range(p, g);
-      pre[g + 1] = (r.y - r.x + kBM - 1) / kBM;
+      const int2 r = group_range(p, g, f);
+      if (!kWgrad) pre[g + 1] = (r.y - r.x + kBM - 1) / kBM;
+      else if (p.G <= kSortGroups) pre[kSortGroups + g] = r.y - r.x;
     }
-    if (threadIdx.x == 0) pre[0] = 0;
+  };
+  bool fall = false;
+  for (int g = threadIdx.x; g < p.G; g += threads_of(MODE)) {
+    const int a = p.offsets[g], b = p.offsets[g + 1];
+    fall |= b < a;
+    if (blockIdx.x == 0 && (a < 0 || b < a || b > p.R)) report_error(p.status, kIndexOutOfRange, g);
+  }
+  sizes(false);
+  if (!kWgrad && threadIdx.x == 0) pre[0] = 0;
+  const bool falls = __syncthreads_or(fall);
+  if (falls) {
+    sizes(true);
     __syncthreads();
+  }
+  if constexpr (!kWgrad) {
     if (warp == 1) {
       int carry = 0;
       for (int g0 = 0; g0 < p.G; g0 += 32) {
@@ -305,34 +336,21 @@ __global__ void __launch_bounds__(threads_of(MODE), 1)
         carry += __shfl_sync(0xffffffffu, v, 31);
       }
     }
-  }
-  if constexpr (MODE == kGroupedWgrad) {
-    if (p.G <= kSortGroups) {  // by falling size, equal ones in order
-      int* size = pre + kSortGroups;
-      for (int g = threadIdx.x; g < p.G; g += threads_of(MODE)) {
-        const int2 r = group_range(p, g);
-        size[g] = r.y - r.x;
-      }
-      __syncthreads();
-      for (int g = threadIdx.x; g < p.G; g += threads_of(MODE)) {
-        const int mine = size[g];
-        int at = 0;
-        for (int o = 0; o < p.G; ++o) at += size[o] > mine || (size[o] == mine && o < g);
-        pre[at] = g;
-      }
+  } else if (p.G <= kSortGroups) {  // by falling size, equal ones in order
+    const int* size = pre + kSortGroups;
+    for (int g = threadIdx.x; g < p.G; g += threads_of(MODE)) {
+      const int mine = size[g];
+      int at = 0;
+      for (int o = 0; o < p.G; ++o) at += size[o] > mine || (size[o] == mine && o < g);
+      pre[at] = g;
     }
-  }
-  if (blockIdx.x == 0) {  // a group that ends before it starts, or outside the rows, is reported
-    for (int g = threadIdx.x; g < p.G; g += threads_of(MODE))
-      if (p.offsets[g] < 0 || p.offsets[g + 1] < p.offsets[g] || p.offsets[g + 1] > p.R)
-        report_error(p.status, kIndexOutOfRange, g);
   }
   sm100::tc_fence_before();
   __syncthreads();
   sm100::tc_fence_after();
   const uint32_t tmem = *slot;
   Tile t;
-  Walk<MODE, BN> walk(p, pre, blockIdx.x, gridDim.x);
+  Walk<MODE, BN> walk(p, pre, blockIdx.x, gridDim.x, falls);
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
@@ -442,7 +460,7 @@ __global__ void __launch_bounds__(threads_of(MODE), 1)
     const int c0 = ((warp - 2) >> 2) * (BN / 2);
     uint8_t* stage = sm + L::kOffEpi + (warp - 2) * 2048;
     float* bias = reinterpret_cast<float*>(sm + L::kOffBias + (warp - 2) * 128);
-    if constexpr (MODE != kGroupedWgrad) zero_outside(p, blockIdx.x * kEpiWarps + warp - 2, gridDim.x * kEpiWarps);
+    if constexpr (MODE != kGroupedWgrad) zero_outside(p, blockIdx.x * kEpiWarps + warp - 2, gridDim.x * kEpiWarps, falls);
     uint32_t i = 0;
     while (walk.next(t)) {
       const int buf = i & 1;
@@ -767,40 +785,60 @@ __global__ void __launch_bounds__(256, 3) few_rows_kernel(GroupedArgs a, int sli
   __shared__ float xs[kFewK][kFewRows];
   __shared__ float part[8][kFewRows][64];
   __shared__ float sum[kFewRows][64];
-  __shared__ int found;
+  __shared__ int found, found_lo, found_hi, top[8];
   const int lane = lane_id();
   const uint32_t rank = blockIdx.z;
   const int R = static_cast<int>(a.R);
   const GP p{a.offsets, a.G, R};
-  if (threadIdx.x < 32) {  // the blockIdx.y-th group with rows
-    int seen = 0, g = -1;
+  if (threadIdx.x < 32) {  // the blockIdx.y-th group with rows, and those rows
+    int seen = 0, g = -1, run = 0;  // run: the largest offset so far, where the next group starts at least
     for (int g0 = 0; g0 < a.G && g < 0; g0 += 32) {
-      const int2 r = g0 + lane < a.G ? group_range(p, g0 + lane) : make_int2(0, 0);
-      const unsigned m = __ballot_sync(0xffffffffu, r.y > r.x);
+      int lo = clamped(p, min(g0 + lane, a.G));
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, lo, o);
+        if (lane >= o) lo = max(lo, up);
+      }
+      lo = max(lo, run);
+      run = __shfl_sync(0xffffffffu, lo, 31);
+      const int hi = max(lo, clamped(p, min(g0 + lane + 1, a.G)));
+      const unsigned m = __ballot_sync(0xffffffffu, hi > lo);
       const int n = __popc(m), want = static_cast<int>(blockIdx.y) - seen;
       if (want < n) {  // the want-th set bit: the lane with that many below it
-        const unsigned hit = __ballot_sync(0xffffffffu, r.y > r.x && __popc(m & ((1u << lane) - 1u)) == want);
-        g = g0 + __ffs(hit) - 1;
+        const bool mine = hi > lo && __popc(m & ((1u << lane) - 1u)) == want;
+        g = g0 + __ffs(__ballot_sync(0xffffffffu, mine)) - 1;
+        if (mine) found_lo = lo, found_hi = hi;
       }
       seen += n;
     }
     if (lane == 0) found = g;
   }
-  if (blockIdx.x == 0 && blockIdx.y == 0 && rank == 0) {
-    for (int g = threadIdx.x; g < a.G; g += 256)
-      if (a.offsets[g] < 0 || a.offsets[g + 1] < a.offsets[g] || a.offsets[g + 1] > R) report_error(a.status, kIndexOutOfRange, g);
-  }
-  if (blockIdx.y == 0 && rank == 0) {  // rows of no group
-    const int first = group_range(p, 0).x, last = group_range(p, a.G - 1).y;
-    for (int i = threadIdx.x; i < R * 64; i += 256) {
-      const int r = i >> 6, c = blockIdx.x * 64 + (i & 63);
-      if ((r < first || r >= last) && c < a.N) store_any(a.out, static_cast<int64_t>(r) * a.N + c, a.out_dtype, 0.f);
+  const bool lead = blockIdx.y == 0 && rank == 0;
+  if (lead) {
+    int last = 0;
+    for (int g = threadIdx.x; g <= a.G; g += 256) last = max(last, clamped(p, g));
+    last = __reduce_max_sync(0xffffffffu, last);
+    if (lane == 0) top[warp_id()] = last;
+    if (blockIdx.x == 0) {
+      for (int g = threadIdx.x; g < a.G; g += 256)
+        if (a.offsets[g] < 0 || a.offsets[g + 1] < a.offsets[g] || a.offsets[g + 1] > R) report_error(a.status, kIndexOutOfRange, g);
     }
   }
   __syncthreads();
+  if (lead) {  // rows of no group
+    int first = clamped(p, 0), last = 0;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) last = max(last, top[q]);
+    if (first > 0 || last < R) {
+      for (int i = threadIdx.x; i < R * 64; i += 256) {
+        const int r = i >> 6, c = blockIdx.x * 64 + (i & 63);
+        if ((r < first || r >= last) && c < a.N) store_any(a.out, static_cast<int64_t>(r) * a.N + c, a.out_dtype, 0.f);
+      }
+    }
+  }
   const int g = found;
   if (g < 0) return;  // every CTA of the cluster
-  const int2 rg = group_range(p, g);
+  const int2 rg = make_int2(found_lo, found_hi);
   const int per = (a.K + slices - 1) / slices, k0 = min(a.K, static_cast<int>(rank) * per), k1 = min(a.K, k0 + per);
   for (int r0 = rg.x; r0 < rg.y; r0 += kFewRows) {
     const int nr = min(kFewRows, rg.y - r0);
@@ -867,7 +905,7 @@ __global__ void __launch_bounds__(256) group_sum_small_kernel(GroupSumArgs a, in
   __shared__ float sum[64];
   const int g = blockIdx.y, lane = lane_id(), warp = warp_id(), c8 = threadIdx.x & 7;
   const uint32_t rank = blockIdx.z;
-  const int2 rg = group_range(GP{a.offsets, a.G, static_cast<int>(a.R)}, g);
+  const int2 rg = group_range_warp(GP{a.offsets, a.G, static_cast<int>(a.R)}, g);
   const int per = (rg.y - rg.x + slices - 1) / slices;
   const int r0 = min(rg.y, rg.x + static_cast<int>(rank) * per), r1 = min(rg.y, r0 + per);
   const int c = blockIdx.x * 64 + c8 * 8;
@@ -911,14 +949,17 @@ __global__ void __launch_bounds__(256) group_part_kernel(GroupSumArgs a, int row
   const GP p{a.offsets, a.G, static_cast<int>(a.R)};
   const int lane = lane_id(), warp = warp_id(), chunk = blockIdx.x;
   const int c0 = chunk * rows, c1 = min(p.R, c0 + rows), c = blockIdx.y * 256 + lane * 8;
-  int lo = 0, hi = a.G;  // the first group that ends behind c0
+  bool fall = false;
+  for (int g = threadIdx.x; g < a.G; g += 256) fall |= a.offsets[g + 1] < a.offsets[g];
+  const bool falls = __syncthreads_or(fall);
+  int lo = 0, hi = falls ? 0 : a.G;  // the first group that ends behind c0 (none is passed over where offsets fall)
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
-    if (group_range(p, mid).y > c0) hi = mid;
+    if (group_range(p, mid, false).y > c0) hi = mid;
     else lo = mid + 1;
   }
   for (int g = lo; g < a.G; ++g) {
-    const int2 rg = group_range(p, g);
+    const int2 rg = group_range(p, g, falls);
     if (rg.x >= c1) break;
     const int r0 = max(rg.x, c0), r1 = min(rg.y, c1);
     if (r0 >= r1) continue;
@@ -946,8 +987,8 @@ __global__ void __launch_bounds__(256) group_part_kernel(GroupSumArgs a, int row
 
 __global__ void __launch_bounds__(256) group_sum_kernel(GroupSumArgs a, int rows) {
   const int g = blockIdx.x, col = blockIdx.y * 256 + threadIdx.x;
+  const int2 rg = group_range_warp(GP{a.offsets, a.G, static_cast<int>(a.R)}, g);
   if (col >= a.N) return;
-  const int2 rg = group_range(GP{a.offsets, a.G, static_cast<int>(a.R)}, g);
   float v = 0.f;
   if (rg.y > rg.x) {
 #pragma unroll 4

@@ -140,7 +140,8 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
     ``[R, in]`` in group order.  ``weight`` is ``[.., in, out]`` with ``groups`` matrices in all, ``bias`` ``[.., out]``;
     they may be float32 (the weight is rounded to x's type; gradients come back in the types of the operands).  On CUDA
     ``x`` is bfloat16 or float16, and ``in`` and ``out`` are multiples of 8.  Returns ``[R, out]``; a row of no group is
-    zero.  Offsets that fall, or leave ``0 .. R``, are clamped and reported by ``default_status(device).check()``.
+    zero.  Offsets that fall, or leave ``0 .. R``, are reported by ``default_status(device).check()``; they are clamped to the rows,
+    and a group starts at the largest offset up to its own: no row belongs to two groups.
 
     Sums are in float32 and rounded once.  For the backward pass the gathered rows and the rounded weight are kept; a
     token's input gradient is summed over its rows in float32.

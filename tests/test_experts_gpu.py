@@ -259,6 +259,39 @@ def test_grouped_linear_bad_offsets_are_reported(cuda):
             st.check("offsets")
 
 
+@pytest.mark.parametrize("R,off", [
+    (12, [0, 7, 2, 12]), (16, [9, 3, 12, 14, -5, 11]), (14, [3] + [(i * 37) % 14 for i in range(80)]), (700, [0, 400, 130, 650, 10, 700]),
+    (700, [650, 20, 300, 900, 100]), (5000, [(i * 977) % 5000 for i in range(601)]), (9000, [0, 8000, 4000, 8500, 100, 9000]),
+    (9000, [(i * 1117) % 9000 for i in range(41)])])
+def test_grouped_linear_falling_offsets_share_no_row(cuda, R, off):
+    """A group starts at the largest offset up to its own, as on the CPU: no row is computed twice, and each call gives the
+    bits that the rising offsets give."""
+    gen = torch.Generator(device="cuda").manual_seed(R)
+    G, top, rising = len(off) - 1, 0, []
+    for o in off:
+        top = max(top, min(max(o, 0), R))
+        rising.append(top)
+    x, dy = torch.randn(R, 40, device=cuda, generator=gen).to(BF16), torch.randn(R, 72, device=cuda, generator=gen).to(BF16)
+    w, b = torch.randn(G, 40, 72, device=cuda, generator=gen).to(BF16), torch.randn(G, 72, device=cuda, generator=gen)
+    st = default_status(cuda)
+    st.check()
+    outs = []
+    for o in (off, rising):
+        leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+        y = grouped_linear(*leaves, offsets=torch.tensor(o, dtype=torch.int32, device=cuda))
+        outs.append((y.detach(), *torch.autograd.grad(y, leaves, dy)))
+        if o is off:
+            with pytest.raises(RuntimeError, match="out of range"):
+                st.check("offsets")
+    st.check()
+    for name, u, v in zip(("y", "dx", "dw", "db"), *outs):
+        assert torch.equal(u, v), name
+    on_cpu = grouped_linear(x.cpu().double(), w.cpu().double(), b.cpu().double(), offsets=torch.tensor(off, dtype=torch.int32))
+    assert torch.equal(on_cpu, grouped_linear(x.cpu().double(), w.cpu().double(), b.cpu().double(), offsets=torch.tensor(rising, dtype=torch.int32)))
+    mag = grouped_linear(x.cpu().double().abs(), w.cpu().double().abs(), b.cpu().double().abs(), offsets=torch.tensor(rising, dtype=torch.int32))
+    within(outs[0][0].cpu(), on_cpu, 43 * 2 ** -23 * mag)
+
+
 @pytest.mark.parametrize("R,G", [(9000, 1), (5000, 3)])
 def test_grouped_linear_in_slices(cuda, R, G):
     """Few groups of a small weight: the weight gradient's rows are cut into slices, written and accumulated."""
