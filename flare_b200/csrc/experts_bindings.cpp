@@ -204,6 +204,7 @@ std::tuple<Tensor, optional<Tensor>> combine_backward(const optional<Tensor>& z,
   p.lddy = pitch(dy);
   Tensor dz = empty({R, N}, dy, dy.scalar_type());
   p.dz = dz.data_ptr();
+  TORCH_CHECK(offsets.numel() >= 1, "combine_rows: offsets without a value");
   p.total = ints(offsets, dy, offsets.numel(), "offsets") + offsets.numel() - 1;
   optional<Tensor> dw;
   if (weights.has_value()) {
@@ -556,6 +557,11 @@ Tensor combine_rows_op(const Tensor& z, const optional<Tensor>& weights, const T
   value_check(z.dim() == 2 && z.size(0) == row_of.numel(), "z must be [", row_of.numel(), ", n] for this route, got ", z.sizes());
   type_check(is_float(z.scalar_type()), "z must be float32, bfloat16 or float16, got ", z.scalar_type());
   same_device(z, row_of);
+  // the gradient of z reads the last offset
+  value_check(offsets.scalar_type() == at::kInt && offsets.dim() == 1 && offsets.size(0) >= 1 && offsets.is_contiguous(),
+              "offsets must be int32 [groups + 1], got ", offsets.scalar_type(), " ", offsets.sizes());
+  same_device(z, offsets);
+  value_check(row_of.scalar_type() == at::kInt && row_of.is_contiguous(), "row_of must be int32 and contiguous, got ", row_of.scalar_type());
   const Tensor v = unit_rows(z);
   optional<Tensor> w;
   if (weights.has_value()) {

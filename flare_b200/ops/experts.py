@@ -256,6 +256,8 @@ def combine_rows(z: torch.Tensor, route: ExpertRoute, weights: torch.Tensor | No
         return native().combine_rows(z, weights, route.offsets, route.row_of)
     if z.dim() != 2 or z.shape[0] != route.row_of.numel():
         raise ValueError(f"z must be [{route.row_of.numel()}, n] for this route, got {tuple(z.shape)}")
+    if route.offsets.dtype != torch.int32 or route.offsets.dim() != 1 or not route.offsets.numel():
+        raise ValueError(f"offsets must be int32 [groups + 1], got {route.offsets.dtype} {tuple(route.offsets.shape)}")
     if weights is not None and weights.numel() != route.row_of.numel():
         raise ValueError(f"weights must have the shape {tuple(route.row_of.shape)}, got {tuple(weights.shape)}")
     on_cuda(z, route.row_of, *(() if weights is None else (weights,)))  # refuses a mixture of devices

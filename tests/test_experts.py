@@ -257,6 +257,23 @@ def test_native_refusals():
             call()
 
 
+def test_combination_checks_the_offsets_of_a_route():
+    """The gradient reads the last offset: a route whose offsets have none, or are of another type, is refused at the call."""
+    from flare_b200._native import available, native
+
+    route = route_topk(torch.randn(4, 3), 2)
+    z = torch.randn(8, 2)
+    for bad in (route.offsets[:0], route.offsets.long(), route.offsets.view(1, -1)):
+        with pytest.raises(ValueError, match="offsets must be int32"):
+            combine_rows(z, route._replace(offsets=bad), route.weights)
+        if available():
+            with pytest.raises(ValueError, match="offsets must be int32"):
+                native().combine_rows(z, route.weights, bad, route.row_of)
+    if available():
+        with pytest.raises(ValueError, match="row_of must be int32"):
+            native().combine_rows(z, route.weights, route.offsets, route.row_of.long())
+
+
 def test_first_call_in_a_capture_is_refused(monkeypatch):
     from flare_b200 import _native
     from flare_b200.ops import experts
