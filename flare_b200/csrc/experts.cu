@@ -387,12 +387,32 @@ void route_bwd_launch(const RouteBwdParams& p, cudaStream_t s) {
 // ------------------------------------------------------------------ SwiGLU
 constexpr int kGroupCols = 32;
 
-// sigmoid: outputs of 16 bits lose nothing to the fast exponential (2 ulp of fp32 and more for
-// large arguments) and division; fp32 outputs take the accurate ones.
+// sigmoid of gates from kTailGate up: outputs of 16 bits lose nothing to the fast exponential (2 ulp
+// of fp32 and more for large arguments) and division; fp32 outputs take the accurate ones.
 template <bool kFast>
 __device__ __forceinline__ float sigmoid_f(float g) {
   if constexpr (kFast) return __fdividef(1.f, 1.f + __expf(-g));
   return 1.f / (1.f + expf(-g));
+}
+
+// Below about -87, exp(-gate) passes fp32's range (and the fast division gives 0 for divisors above
+// 2^126), but up and dy can be as large as the sigmoid is small: with up = 1e36 and a gate of -89 the
+// result is -0.2.  Such gates are rare; their products are taken in 64 bits, value by value from
+// memory and over what the vector store wrote (with the operands kept in registers for it, the
+// backward kernel took 72 of them instead of 48, and a pass of 131072 x 2 x 2048 bf16 844 us instead
+// of 737).  sigmoid(g) is exp(g) there (1 + exp(g) rounds to 1), and exp(g) the eighth power of
+// expf(g / 8), which is a normal number down to -698: off by 8 ulp of fp32 at most.
+constexpr float kTailGate = -80.f;
+__device__ __forceinline__ double tail_sigmoid(float g) {
+  const double e = expf(0.125f * g), e2 = e * e, e4 = e2 * e2;
+  return e4 * e4;
+}
+template <int N>
+__device__ __forceinline__ bool has_tail(const float (&gate)[N]) {
+  float low = gate[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) low = fminf(low, gate[i]);  // fminf passes over NaN
+  return low < kTailGate;
 }
 
 // The scale exponent of a group whose largest finite magnitude is `top`: the largest value lands
@@ -488,7 +508,15 @@ __global__ void __launch_bounds__(256) swiglu_fwd_kernel(SwigluParams p, RowTili
         float y[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) y[i] = up[i] * (gate[i] * sigmoid_f<sizeof(T) == 2>(gate[i]));
-        store_f<T, N>(static_cast<T*>(p.y) + r * p.h + col, y);
+        T* out = static_cast<T*>(p.y) + r * p.h + col;
+        store_f<T, N>(out, y);
+        if (has_tail(gate)) {
+#pragma unroll 1
+          for (int i = 0; i < N; ++i) {
+            const float g = to_f32(x[p.h + i]);
+            if (g < kTailGate) out[i] = from_f32<T>(static_cast<float>(to_f32(x[i]) * (g * tail_sigmoid(g))));
+          }
+        }
       }
       if constexpr (kKeep) {
         bool iu, ig;
@@ -516,9 +544,9 @@ __global__ void __launch_bounds__(256) swiglu_fwd_kernel(SwigluParams p, RowTili
 
 // d up = dy * gate * s, d gate = dy * up * s * (1 + gate * (1 - s)), s = sigmoid(gate), from x
 // itself or from the values that the checkpoint stands for.  The factors of s come first: a large
-// negative gate makes them 0 before the others can overflow.
+// negative gate makes them 0 before the others can overflow.  Five blocks an SM: 48 registers.
 template <typename T, int N, bool kKeep>
-__global__ void __launch_bounds__(256) swiglu_bwd_kernel(SwigluParams p, RowTiling t) {
+__global__ void __launch_bounds__(256, 5) swiglu_bwd_kernel(SwigluParams p, RowTiling t) {
   constexpr int GL = kGroupCols / N;
   const int r0 = t.rows > 1 ? threadIdx.x / t.cols : 0;
   const int c0 = t.rows > 1 ? threadIdx.x % t.cols : threadIdx.x;
@@ -541,6 +569,7 @@ __global__ void __launch_bounds__(256) swiglu_bwd_kernel(SwigluParams p, RowTili
         load_f<T, N>(x + p.h, gate);
       }
       load_f<T, N>(static_cast<const T*>(p.dy) + r * p.lddy + col, dy);
+      const bool tail = has_tail(gate);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const float s = sigmoid_f<sizeof(T) == 2>(gate[i]);
@@ -550,6 +579,27 @@ __global__ void __launch_bounds__(256) swiglu_bwd_kernel(SwigluParams p, RowTili
       T* dx = static_cast<T*>(p.dx) + r * 2 * p.h + col;
       store_f<T, N>(dx, du);
       store_f<T, N>(dx + p.h, dg);
+      if (tail) {
+#pragma unroll 1
+        for (int i = 0; i < N; ++i) {
+          float u[1], g[1];
+          if constexpr (kKeep) {
+            const uint8_t* q = p.q + r * 2 * p.h + col + i;
+            const uint8_t* sc = p.scale + r * 2 * groups + c / GL;
+            unpack_e4m3<1>(q, exp2_int(static_cast<int>(sc[0]) - 127), u);
+            unpack_e4m3<1>(q + p.h, exp2_int(static_cast<int>(sc[groups]) - 127), g);
+          } else {
+            const T* x = static_cast<const T*>(p.x) + r * p.ldx + col + i;
+            load_f<T, 1>(x, u);
+            load_f<T, 1>(x + p.h, g);
+          }
+          if (g[0] < kTailGate) {
+            const double d = to_f32(static_cast<const T*>(p.dy)[r * p.lddy + col + i]), s = tail_sigmoid(g[0]);
+            dx[i] = from_f32<T>(static_cast<float>(d * (g[0] * s)));
+            dx[p.h + i] = from_f32<T>(static_cast<float>(d * (u[0] * (s * (1.0 + g[0])))));
+          }
+        }
+      }
     }
   }
 }

@@ -193,7 +193,7 @@ def e4m3_checkpoint_reference(x: torch.Tensor) -> torch.Tensor:
 
 def _swiglu_plain(x):
     h = x.shape[1] // 2
-    xf = x if x.dtype == torch.float64 else x.float()
+    xf = x.double()  # a sigmoid below float32's range times a large value need not be small
     up, gate = xf[:, :h], xf[:, h:]
     return (up * (gate * torch.sigmoid(gate))).to(x.dtype)
 

@@ -141,6 +141,15 @@ def test_swiglu_gradient_is_the_formula_at_the_checkpoint():
         torch.testing.assert_close(leaf.grad, at.grad)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_swiglu_gates_whose_sigmoid_leaves_float32(dtype):
+    gate = -torch.linspace(80, 110, 61)
+    x = torch.cat([torch.full_like(gate, 1e36), gate]).view(1, -1).to(dtype)
+    up, g = x[:, :61].double(), x[:, 61:].double()
+    want = up * g * torch.exp(g)
+    torch.testing.assert_close(swiglu(x).double(), want, rtol=torch.finfo(dtype).eps / 2 + 1e-12, atol=0)
+
+
 @pytest.mark.parametrize("slots", [1, 3])
 def test_expert_mlp_matches_all_experts_then_pick(slots):
     """The routed block against the sparse layer that computes every expert, outputs and gradients, in 64 bits."""

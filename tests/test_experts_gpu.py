@@ -397,6 +397,40 @@ def test_swiglu_extremes(cuda):
     assert torch.equal(dx.isnan(), dwant.isnan())
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("checkpoint", [None, "e4m3"])
+@pytest.mark.parametrize("h", [64, 37])
+def test_swiglu_gates_whose_sigmoid_leaves_float32(cuda, h, checkpoint, dtype):
+    """Gates from -78 down, where the sigmoid is below float32's normal range but its product with up or dy is not."""
+    big = 3e4 if dtype == FP16 else 1e36
+    gen = torch.Generator(device="cuda").manual_seed(h)
+    gate = -torch.linspace(78, 110, 40 * h, device=cuda).view(40, h)
+    gate[-1] = -torch.linspace(110, 700, h, device=cuda)
+    gate[::3, ::2] = torch.randn(14, (h + 1) // 2, device=cuda, generator=gen)  # ordinary ones beside them
+    up = big * torch.randn(40, h, device=cuda, generator=gen)
+    x, dy = torch.cat([up, gate], 1).to(dtype), (big * torch.randn(40, h, device=cuda, generator=gen)).to(dtype)
+    if dtype != FP16:
+        dy[:, 1::2] = torch.randn(40, h // 2, device=cuda, generator=gen).to(dtype)
+        dy[::3, ::2] = 1.0  # ordinary gates: results within the type's range
+    leaf = x.clone().requires_grad_(True)
+    y = swiglu(leaf, checkpoint=checkpoint)
+    dx, = torch.autograd.grad(y, leaf, dy)
+    at = e4m3_checkpoint_reference(x.cpu()).to(cuda) if checkpoint else x
+    want, dwant = exact_swiglu(x, dy)[0], exact_swiglu(at, dy)[1]
+    most = torch.finfo(dtype).max
+    def slack(v):  # as in test_swiglu; 8 steps for the eighth power and five roundings where the 64-bit form is taken
+        return (13 + 2 * v[:, h:].double().abs().clamp(max=100)) * 2 ** -23
+    ok = want.abs() < most
+    within(y.detach()[ok], want[ok], (slack(x) * want.abs())[ok], "y")
+    g, d, u = at[:, h:].double(), dy.double(), at[:, :h].double()
+    s = torch.sigmoid(g)
+    mag = torch.cat([(d * g * s).abs(), (d * u * s).abs() * (1 + g.abs())], 1)
+    ok = dwant.abs() < most * 0.99
+    within(dx[ok], dwant[ok], (2 * slack(at).repeat(1, 2) * mag)[ok], "dx")
+    if dtype != FP16 and checkpoint is None:  # what is tested here: results that are not small
+        assert int(((want.abs() > 1e-3) & (x[:, h:] < -88)).sum()) > h
+
+
 def test_swiglu_views(cuda):
     base = torch.randn(50, 300, device=cuda).to(BF16)
     for x in (base[:, 4:132], base[:, 3:131], base[::2, 8:72], base.t()[:128].t(), base[:1, :64].expand(9, 64)):
