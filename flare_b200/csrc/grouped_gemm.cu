@@ -83,29 +83,44 @@ struct Smem {
   static constexpr int kOffEpi = kOffB + STAGES * kTileB;       // 2 KiB per epilogue warp
   static constexpr int kOffBias = kOffEpi + kEpiWarps * 2048;   // 32 floats per epilogue warp
   static constexpr int kOffPre = kOffBias + kEpiWarps * 128;    // tile prefix of the groups, or their order
-  static constexpr int kOffBar = kOffPre + (kGroupedMaxGroups + 2) * 4;
+  static constexpr int kOffOff = kOffPre + (kGroupedMaxGroups + 2) * 4;  // offsets
+  static constexpr int kOffBar = kOffOff + (kGroupedMaxGroups + 2) * 4;
   static constexpr int kBytes = kOffBar + (3 * STAGES + 4) * 8 + 16;
   static constexpr int kAlloc = kBytes + 1024;
   static_assert(kOffBar % 8 == 0, "barriers are 8-byte aligned");
   static_assert(kAlloc <= 227 * 1024, "shared memory of one CTA");
 };
 
-// Rows of group g: offsets are clamped to the rows, and a group starts at the largest offset up to
-// its own, so that no two groups share a row whatever the offsets are (a row that two had would be
-// written by two CTAs).  Where the offsets rise, that is its own offset: `falls` says that they do not.
+// Offsets are clamped to the rows, and a group starts at the largest offset up to its own, so that no
+// two groups share a row whatever the offsets are (a row that two had would be written by two CTAs).
 __device__ __forceinline__ int clamped(const GP& p, int g) { return min(max(p.offsets[g], 0), p.R); }
-__device__ __forceinline__ int2 group_range(const GP& p, int g, bool falls) {
-  int lo = clamped(p, g);
-  if (falls)
-    for (int o = 0; o < g; ++o) lo = max(lo, clamped(p, o));
-  return make_int2(lo, max(lo, clamped(p, g + 1)));
+
+// The same rising offsets off[0 .. G] in shared memory, by a whole block of n threads.  Whether there
+// were any that fell.
+__device__ __forceinline__ bool load_offsets(const GP& p, int* off, int n) {
+  bool fall = false;
+  for (int g = threadIdx.x; g <= p.G; g += n) {
+    const int a = p.offsets[g];
+    off[g] = min(max(a, 0), p.R);
+    fall |= p.offsets[min(g + 1, p.G)] < a;
+  }
+  fall = __syncthreads_or(fall);
+  if (fall) {
+    if (threadIdx.x == 0)
+      for (int g = 1; g <= p.G; ++g) off[g] = max(off[g], off[g - 1]);
+    __syncthreads();
+  }
+  return fall;
 }
-// The same by a whole warp, which needs no flag (32 offsets at a time).
+
+// The rows of one group by a whole warp, straight from the offsets: all of its loads at once.
 __device__ __forceinline__ int2 group_range_warp(const GP& p, int g) {
-  int lo = 0;
-  for (int o = lane_id(); o <= g; o += 32) lo = max(lo, clamped(p, o));
-  lo = __reduce_max_sync(0xffffffffu, lo);
-  return make_int2(lo, max(lo, clamped(p, g + 1)));
+  int lo = clamped(p, g);
+  const int hi = clamped(p, g + 1);
+  int top = lane_id() < g ? clamped(p, lane_id()) : 0;
+  for (int o = lane_id() + 32; o < g; o += 32) top = max(top, clamped(p, o));
+  if (__any_sync(0xffffffffu, top > lo)) lo = max(lo, __reduce_max_sync(0xffffffffu, top));
+  return make_int2(lo, max(lo, hi));
 }
 
 struct Tile {
@@ -122,12 +137,11 @@ constexpr int kSortGroups = 512;
 template <int MODE, int BN>
 struct Walk {
   const GP& p;
-  const int* pre;
+  const int *off, *pre;
   int turn, me, step, total, g;
-  bool falls;
-  __device__ Walk(const GP& p_, const int* pre_, int first, int step_, bool falls_)
-      : p(p_), pre(pre_), turn(0), me(first), step(step_),
-        total(MODE == kGroupedWgrad ? p_.G * p_.mt * p_.nt * p_.slices : pre_[p_.G] * p_.nt), g(0), falls(falls_) {}
+  __device__ Walk(const GP& p_, const int* off_, const int* pre_, int first, int step_)
+      : p(p_), off(off_), pre(pre_), turn(0), me(first), step(step_),
+        total(MODE == kGroupedWgrad ? p_.G * p_.mt * p_.nt * p_.slices : pre_[p_.G] * p_.nt), g(0) {}
   __device__ bool next(Tile& t) {
     int u = turn * step + me;
     if (MODE == kGroupedWgrad && (turn & 1)) u = turn * step + (step - 1 - me);
@@ -143,7 +157,7 @@ struct Walk {
       t.slice = m / p.mt;
       m -= t.slice * p.mt;
       t.g = p.G <= kSortGroups ? pre[at] : at;
-      const int2 r = group_range(p, t.g, falls);
+      const int2 r = make_int2(off[t.g], off[t.g + 1]);
       t.m0 = m * kBM;
       const int steps = (r.y - r.x + kBK - 1) / kBK;
       const int s0 = static_cast<int>(static_cast<int64_t>(steps) * t.slice / p.slices);
@@ -154,7 +168,7 @@ struct Walk {
     } else {
       while (pre[g + 1] <= m) ++g;
       m -= pre[g];
-      const int2 r = group_range(p, g, falls);
+      const int2 r = make_int2(off[g], off[g + 1]);
       t.g = g;
       t.lo = r.x;
       t.hi = r.y;
@@ -241,9 +255,9 @@ __device__ __forceinline__ void regs_ready(uint32_t (&r)[32]) {
 }
 
 // Rows outside every group (before the first, behind the last) become zeros.
-__device__ __forceinline__ void zero_outside(const GP& p, int warp, int warps, bool falls) {
+__device__ __forceinline__ void zero_outside(const GP& p, const int* off, int warp, int warps) {
   const int lane = lane_id();
-  const int first = clamped(p, 0), last = group_range(p, p.G - 1, falls).y;
+  const int first = off[0], last = off[p.G];
   const int64_t n = static_cast<int64_t>(first) + (p.R - last);
   for (int64_t i = warp; i < n; i += warps) {
     const int64_t r = i < first ? i : last + (i - first);
@@ -273,6 +287,7 @@ __global__ void __launch_bounds__(threads_of(MODE), 1)
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* sm = smem_raw + (((raw + 1023u) & ~1023u) - raw);
   int* pre = reinterpret_cast<int*>(sm + L::kOffPre);
+  int* off = reinterpret_cast<int*>(sm + L::kOffOff);
   uint64_t* full = reinterpret_cast<uint64_t*>(sm + L::kOffBar);
   uint64_t* empty = full + STAGES;
   uint64_t* tail = empty + STAGES;  // a partial step has landed in this CTA
@@ -299,34 +314,13 @@ __global__ void __launch_bounds__(threads_of(MODE), 1)
     sm100::tmem_alloc(slot, 2 * BN);
     sm100::tmem_relinquish();
   }
-  // A group that ends before it starts, or outside the rows, is reported by the first CTA; every one
-  // has to know of those that fall.  pre: tiles of the groups, or (weight gradient) their sizes.
-  constexpr bool kWgrad = MODE == kGroupedWgrad;
-  auto sizes = [&](bool f) {
-    for (int g = threadIdx.x; g < p.G; g += threads_of(MODE)) {
-      const int2 r = group_range(p, g, f);
-      if (!kWgrad) pre[g + 1] = (r.y - r.x + kBM - 1) / kBM;
-      else if (p.G <= kSortGroups) pre[kSortGroups + g] = r.y - r.x;
-    }
-  };
-  bool fall = false;
-  for (int g = threadIdx.x; g < p.G; g += threads_of(MODE)) {
-    const int a = p.offsets[g], b = p.offsets[g + 1];
-    fall |= b < a;
-    if (blockIdx.x == 0 && (a < 0 || b < a || b > p.R)) report_error(p.status, kIndexOutOfRange, g);
-  }
-  sizes(false);
-  if (!kWgrad && threadIdx.x == 0) pre[0] = 0;
-  const bool falls = __syncthreads_or(fall);
-  if (falls) {
-    sizes(true);
-    __syncthreads();
-  }
-  if constexpr (!kWgrad) {
+  load_offsets(p, off, threads_of(MODE));
+  if constexpr (MODE != kGroupedWgrad) {
     if (warp == 1) {
+      if (lane == 0) pre[0] = 0;
       int carry = 0;
       for (int g0 = 0; g0 < p.G; g0 += 32) {
-        int v = g0 + lane < p.G ? pre[g0 + lane + 1] : 0;
+        int v = g0 + lane < p.G ? (off[g0 + lane + 1] - off[g0 + lane] + kBM - 1) / kBM : 0;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
           const int up = __shfl_up_sync(0xffffffffu, v, o);
@@ -337,20 +331,30 @@ __global__ void __launch_bounds__(threads_of(MODE), 1)
       }
     }
   } else if (p.G <= kSortGroups) {  // by falling size, equal ones in order
-    const int* size = pre + kSortGroups;
     for (int g = threadIdx.x; g < p.G; g += threads_of(MODE)) {
-      const int mine = size[g];
+      const int mine = off[g + 1] - off[g];
       int at = 0;
-      for (int o = 0; o < p.G; ++o) at += size[o] > mine || (size[o] == mine && o < g);
+      for (int o = 0, from = off[0]; o < p.G; ++o) {
+        const int to = off[o + 1], size = to - from;
+        at += size > mine || (size == mine && o < g);
+        from = to;
+      }
       pre[at] = g;
     }
+  }
+  // A group that ends before it starts, or outside the rows, is reported.  (In load_offsets, in front
+  // of everything else, this cost the forward product of 96 short groups 5 us of 90.)
+  if (blockIdx.x == 0) {
+    for (int g = threadIdx.x; g < p.G; g += threads_of(MODE))
+      if (p.offsets[g] < 0 || p.offsets[g + 1] < p.offsets[g] || p.offsets[g + 1] > p.R)
+        report_error(p.status, kIndexOutOfRange, g);
   }
   sm100::tc_fence_before();
   __syncthreads();
   sm100::tc_fence_after();
   const uint32_t tmem = *slot;
   Tile t;
-  Walk<MODE, BN> walk(p, pre, blockIdx.x, gridDim.x, falls);
+  Walk<MODE, BN> walk(p, off, pre, blockIdx.x, gridDim.x);
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
@@ -460,7 +464,7 @@ __global__ void __launch_bounds__(threads_of(MODE), 1)
     const int c0 = ((warp - 2) >> 2) * (BN / 2);
     uint8_t* stage = sm + L::kOffEpi + (warp - 2) * 2048;
     float* bias = reinterpret_cast<float*>(sm + L::kOffBias + (warp - 2) * 128);
-    if constexpr (MODE != kGroupedWgrad) zero_outside(p, blockIdx.x * kEpiWarps + warp - 2, gridDim.x * kEpiWarps, falls);
+    if constexpr (MODE != kGroupedWgrad) zero_outside(p, off, blockIdx.x * kEpiWarps + warp - 2, gridDim.x * kEpiWarps);
     uint32_t i = 0;
     while (walk.next(t)) {
       const int buf = i & 1;
@@ -905,20 +909,29 @@ __global__ void __launch_bounds__(256) group_sum_small_kernel(GroupSumArgs a, in
   __shared__ float sum[64];
   const int g = blockIdx.y, lane = lane_id(), warp = warp_id(), c8 = threadIdx.x & 7;
   const uint32_t rank = blockIdx.z;
-  const int2 rg = group_range_warp(GP{a.offsets, a.G, static_cast<int>(a.R)}, g);
-  const int per = (rg.y - rg.x + slices - 1) / slices;
-  const int r0 = min(rg.y, rg.x + static_cast<int>(rank) * per), r1 = min(rg.y, r0 + per);
+  const GP p{a.offsets, a.G, static_cast<int>(a.R)};
   const int c = blockIdx.x * 64 + c8 * 8;
-  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (c < a.N) {
-#pragma unroll 8
-    for (int r = r0 + (threadIdx.x >> 3); r < r1; r += 32) {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.y) + r * a.ldy + c));
-      const T* v = reinterpret_cast<const T*>(&u);
+  float acc[8];
+  auto add = [&](int2 rg) {
+    const int per = (rg.y - rg.x + slices - 1) / slices;
+    const int r0 = min(rg.y, rg.x + static_cast<int>(rank) * per), r1 = min(rg.y, r0 + per);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) acc[i] += to_f32(v[i]);
+    for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+    if (c < a.N) {
+#pragma unroll 8
+      for (int r = r0 + (threadIdx.x >> 3); r < r1; r += 32) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.y) + r * a.ldy + c));
+        const T* v = reinterpret_cast<const T*>(&u);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] += to_f32(v[i]);
+      }
     }
-  }
+  };
+  // the group's own offsets, and once more where an earlier one is larger (in one, 6.2 us instead of 5.0)
+  const int2 own = make_int2(clamped(p, g), max(clamped(p, g), clamped(p, g + 1)));
+  add(own);
+  const int2 rg = group_range_warp(p, g);
+  if (rg.x != own.x) add(rg);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], 8);
@@ -946,43 +959,48 @@ __global__ void __launch_bounds__(256) group_sum_small_kernel(GroupSumArgs a, in
 template <typename T>
 __global__ void __launch_bounds__(256) group_part_kernel(GroupSumArgs a, int rows) {
   __shared__ float red[8][256];
+  extern __shared__ int off[];  // [G + 1]
   const GP p{a.offsets, a.G, static_cast<int>(a.R)};
   const int lane = lane_id(), warp = warp_id(), chunk = blockIdx.x;
   const int c0 = chunk * rows, c1 = min(p.R, c0 + rows), c = blockIdx.y * 256 + lane * 8;
-  bool fall = false;
-  for (int g = threadIdx.x; g < a.G; g += 256) fall |= a.offsets[g + 1] < a.offsets[g];
-  const bool falls = __syncthreads_or(fall);
-  int lo = 0, hi = falls ? 0 : a.G;  // the first group that ends behind c0 (none is passed over where offsets fall)
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (group_range(p, mid, false).y > c0) hi = mid;
-    else lo = mid + 1;
-  }
-  for (int g = lo; g < a.G; ++g) {
-    const int2 rg = group_range(p, g, falls);
-    if (rg.x >= c1) break;
-    const int r0 = max(rg.x, c0), r1 = min(rg.y, c1);
-    if (r0 >= r1) continue;
-    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (c < a.N) {
-#pragma unroll 8
-      for (int r = r0 + warp; r < r1; r += 8) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.y) + r * a.ldy + c));
-        const T* v = reinterpret_cast<const T*>(&u);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) acc[i] += to_f32(v[i]);
-      }
+  const bool falls = load_offsets(p, off, 256);
+  auto sums = [&](auto range) {
+    int lo = 0, hi = a.G;  // the first group that ends behind c0
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (off[mid + 1] > c0) hi = mid;
+      else lo = mid + 1;
     }
-    __syncthreads();
+    for (int g = lo; g < a.G; ++g) {
+      const int2 rg = range(g);
+      if (rg.x >= c1) break;
+      const int r0 = max(rg.x, c0), r1 = min(rg.y, c1);
+      if (r0 >= r1) continue;
+      float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (c < a.N) {
+#pragma unroll 8
+        for (int r = r0 + warp; r < r1; r += 8) {
+          const uint4 u = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.y) + r * a.ldy + c));
+          const T* v = reinterpret_cast<const T*>(&u);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) red[warp][lane * 8 + i] = acc[i];
-    __syncthreads();
-    const int col = blockIdx.y * 256 + threadIdx.x;
-    float v = 0.f;
+          for (int i = 0; i < 8; ++i) acc[i] += to_f32(v[i]);
+        }
+      }
+      __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v += red[i][threadIdx.x];
-    if (col < a.N) a.work[static_cast<int64_t>(chunk + g) * a.N + col] = v;
-  }
+      for (int i = 0; i < 8; ++i) red[warp][lane * 8 + i] = acc[i];
+      __syncthreads();
+      const int col = blockIdx.y * 256 + threadIdx.x;
+      float v = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v += red[i][threadIdx.x];
+      if (col < a.N) a.work[static_cast<int64_t>(chunk + g) * a.N + col] = v;
+    }
+  };
+  // The rows of a group are read from the offsets themselves where these rise: with the ones in shared
+  // memory as bounds of the loop, 131072 x 4096 took 190 us instead of 170.
+  if (falls) sums([&](int g) { return make_int2(off[g], off[g + 1]); });
+  else sums([&](int g) { return make_int2(clamped(p, g), clamped(p, g + 1)); });
 }
 
 __global__ void __launch_bounds__(256) group_sum_kernel(GroupSumArgs a, int rows) {
@@ -1040,6 +1058,7 @@ int64_t group_sum_work_floats(int G, int64_t R, int N) {
 }
 
 void group_colsum(const GroupSumArgs& a, cudaStream_t s) {
+  FLARE_CHECK(a.G > 0 && a.G <= kGroupedMaxGroups, "grouped products: 1 to 2048 groups");
   if (a.R <= kSumOneLaunch) {
     const int cols = ceil_div(a.N, 64), slices = slices_for(static_cast<int64_t>(a.G) * cols, a.R / a.G, 128);
     const dim3 grid(cols, a.G, slices);
@@ -1049,8 +1068,9 @@ void group_colsum(const GroupSumArgs& a, cudaStream_t s) {
   }
   const int cols = ceil_div(a.N, 256), rows = sum_rows(a.R, cols);
   const dim3 grid(ceil_div(a.R, rows), cols);
-  if (a.dtype == kBF16) group_part_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(a, rows);
-  else group_part_kernel<__half><<<grid, 256, 0, s>>>(a, rows);
+  const int smem = (a.G + 1) * 4;
+  if (a.dtype == kBF16) group_part_kernel<__nv_bfloat16><<<grid, 256, smem, s>>>(a, rows);
+  else group_part_kernel<__half><<<grid, 256, smem, s>>>(a, rows);
   FLARE_CUDA_CHECK(cudaGetLastError());
   group_sum_kernel<<<dim3(a.G, cols), 256, 0, s>>>(a, rows);
   FLARE_CUDA_CHECK(cudaGetLastError());
