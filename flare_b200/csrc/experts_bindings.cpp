@@ -358,6 +358,10 @@ void group_sums(const Tensor& dy, const Tensor& offsets, const Tensor& db, bool 
 void once(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, " has no second derivative");
 }
+// A forward-mode tangent would be lost: the kernels see values only, and the result would have none.
+void no_tangent(const char* what, const Tensor& t) {
+  if (t._fw_grad(0).defined()) throw std::runtime_error(std::string(what) + " has no forward-mode derivative");
+}
 bool wants(std::initializer_list<const Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : ts)
@@ -528,6 +532,7 @@ py::tuple route_topk_op(const Tensor& logits, int64_t k) {
               flare::kRouteMaxTopK, ", got ", k);
   value_check(E <= flare::kRouteMaxExperts, "at most ", flare::kRouteMaxExperts, " experts a slot, got ", E);
   type_check(is_float(logits.scalar_type()), "logits must be float32, bfloat16 or float16, got ", logits.scalar_type());
+  no_tangent("route_topk", logits);
   const bool flat = logits.dim() == 2;
   Tensor lg = flat ? logits.unsqueeze(0) : logits;
   if (lg.stride(2) != 1 && E > 1) lg = lg.contiguous();
@@ -547,6 +552,7 @@ py::tuple route_topk_op(const Tensor& logits, int64_t k) {
 Tensor swiglu_op(const Tensor& x, bool keep) {
   value_check(x.dim() == 2 && x.size(1) % 2 == 0, "x must be [rows, 2h], got ", x.sizes());
   type_check(is_float(x.scalar_type()), "x must be float32, bfloat16 or float16, got ", x.scalar_type());
+  no_tangent("swiglu", x);
   const Tensor v = unit_rows(x);
   if (wants({&v})) return SwigluFn::apply(v, keep);
   return std::get<0>(swiglu_forward(v, false));
@@ -562,6 +568,8 @@ Tensor combine_rows_op(const Tensor& z, const optional<Tensor>& weights, const T
               "offsets must be int32 [groups + 1], got ", offsets.scalar_type(), " ", offsets.sizes());
   same_device(z, offsets);
   value_check(row_of.scalar_type() == at::kInt && row_of.is_contiguous(), "row_of must be int32 and contiguous, got ", row_of.scalar_type());
+  no_tangent("combine_rows", z);
+  if (weights.has_value()) no_tangent("combine_rows", *weights);
   const Tensor v = unit_rows(z);
   optional<Tensor> w;
   if (weights.has_value()) {
@@ -601,6 +609,9 @@ Tensor grouped_linear_op(const Tensor& x, const Tensor& weight, const optional<T
     type_check(is_float(bias->scalar_type()), "bias must be float32, bfloat16 or float16, got ", bias->scalar_type());
     same_device(x, *bias);
   }
+  no_tangent("grouped_linear", x);
+  no_tangent("grouped_linear", weight);
+  if (bias.has_value()) no_tangent("grouped_linear", *bias);
   const Tensor v = tma_rows(x);
   optional<Tensor> b;
   if (bias.has_value()) b = bias->contiguous();

@@ -283,6 +283,31 @@ def test_combination_checks_the_offsets_of_a_route():
             native().combine_rows(z, route.weights, route.offsets, route.row_of.long())
 
 
+def test_native_refusals_of_tangents():
+    """A forward-mode tangent is refused, not dropped: with or without a gradient, on any operand."""
+    from torch.autograd import forward_ad
+
+    from flare_b200._native import available, native
+
+    if not available():
+        pytest.skip("the native extension is not built")
+    C = native()
+    x, w, b, off = torch.zeros(4, 16).bfloat16(), torch.zeros(3, 16, 24).bfloat16(), torch.zeros(3, 24).bfloat16(), torch.zeros(4, dtype=torch.int32)
+    z, row_of, weights = torch.zeros(8, 16), torch.zeros(4, 2, dtype=torch.int32), torch.zeros(4, 2)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        for leaf in (False, True):
+            for call in (lambda t: C.route_topk(dual(t(x)), 2), lambda t: C.swiglu(dual(t(x)), False), lambda t: C.swiglu(dual(t(x)), True),
+                         lambda t: C.combine_rows(dual(t(z)), weights, off, row_of), lambda t: C.combine_rows(z, dual(t(weights)), off, row_of),
+                         lambda t: C.grouped_linear(dual(t(x)), w, b, off, None, None, None, None, 0, 0),
+                         lambda t: C.grouped_linear(x, dual(t(w)), b, off, None, None, None, None, 0, 0),
+                         lambda t: C.grouped_linear(x, w, dual(t(b)), off, None, None, None, None, 0, 0)):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call(lambda v: v.clone().requires_grad_(leaf))
+
+
 def test_first_call_in_a_capture_is_refused(monkeypatch):
     from flare_b200 import _native
     from flare_b200.ops import experts

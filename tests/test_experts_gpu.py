@@ -712,3 +712,20 @@ def test_refusals(cuda):
     for y in (grouped_linear(leaf, w.to(BF16), route=route), swiglu(leaf), swiglu(leaf, checkpoint="e4m3")):
         with pytest.raises(RuntimeError, match="second derivative"):
             torch.autograd.grad(y.float().sum(), leaf, create_graph=True)
+
+
+def test_tangents_are_refused(cuda):
+    from torch.autograd import forward_ad
+
+    lg, x, w = torch.randn(4, 3, device=cuda), torch.randn(4, 16, device=cuda).to(BF16), torch.randn(3, 16, 24, device=cuda).to(BF16)
+    route = route_topk(lg, 2)
+    z = torch.randn(8, 16, device=cuda)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        for call in (lambda: route_topk(dual(lg), 2), lambda: swiglu(dual(x)), lambda: swiglu(dual(x), checkpoint="e4m3"),
+                     lambda: grouped_linear(dual(x), w, route=route), lambda: grouped_linear(x, dual(w), offsets=torch.zeros(4, dtype=torch.int32, device=cuda)),
+                     lambda: combine_rows(z, route, dual(route.weights)), lambda: combine_rows(dual(z), route)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
