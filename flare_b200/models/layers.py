@@ -28,7 +28,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from ..ops.dense import colsum_
-from ..ops.experts import expert_mlp
+from ..ops.experts import expert_mlp, swiglu
 from ..ops.gemm import gemm
 from ..ops.mixing import gate_mix, relu_bwd_colsum_
 
@@ -460,7 +460,8 @@ class BatchedExpertMoE(nn.Module):
     Input ``x`` is [slots, batch, in_dim]; every slot has its own experts.  ``routed`` (with ``sparse``) computes
     only the chosen experts of every token (``ops.experts.expert_mlp``: routing, grouped products, combination) instead
     of all of them; on CUDA x is then bf16 or fp16.  ``checkpoint="e4m3"`` (with ``routed``) keeps the experts' input
-    activations in 8 bits for the backward pass.
+    activations in 8 bits for the backward pass.  With one expert there is nothing to route: its products are the dense
+    ones, in x's type (float32 too) and of any width, and the checkpoint is kept as asked.
     """
 
     def __init__(self, batch_dim: int, in_dim: int, scale_size: int, num_experts: int, sparse: bool, top_k: int,
@@ -495,10 +496,17 @@ class BatchedExpertMoE(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if self.routed and self.num_experts > 1:
             return self._forward_routed(x)
-        up_gate = torch.einsum("dbi,deih->dbeh", x, self.w_up) + self.b_up.unsqueeze(1)
-        up, gate = up_gate.chunk(2, -1)
-        hidden = F.silu(gate) * up
-        outs = torch.einsum("dbeh,dehi->dbei", hidden, self.w_down) + self.b_down.unsqueeze(1)
+        params = (self.w_up, self.b_up, self.w_down, self.b_down)
+        w_up, b_up, w_down, b_down = (p.to(x.dtype) for p in params) if self.routed else params
+        up_gate = torch.einsum("dbi,deih->dbeh", x, w_up) + b_up.unsqueeze(1)
+        if self.checkpoint is not None:
+            hidden = swiglu(up_gate.reshape(-1, up_gate.shape[-1]), checkpoint=self.checkpoint)
+            hidden = hidden.view(*up_gate.shape[:-1], w_down.shape[-2])
+            del up_gate
+        else:
+            up, gate = up_gate.chunk(2, -1)
+            hidden = F.silu(gate) * up
+        outs = torch.einsum("dbeh,dehi->dbei", hidden, w_down) + b_down.unsqueeze(1)
         if self.num_experts == 1:
             moe = outs[:, :, 0]
         else:
@@ -511,7 +519,8 @@ class BatchedExpertMoE(nn.Module):
             else:
                 moe = (outs * fp32_softmax(logits, -1).unsqueeze(-1)).sum(2)
         if self.residual_norm:
-            return fp32_rms_normalize(x + moe, -1) * self.norm_scale.unsqueeze(1)
+            y = fp32_rms_normalize(x + moe, -1) * self.norm_scale.unsqueeze(1)
+            return y.to(x.dtype) if self.routed else y
         return moe
 
 

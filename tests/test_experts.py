@@ -184,6 +184,61 @@ def test_token_mixers_pass_the_option_on():
         torch.testing.assert_close(b(x), a(x), rtol=1e-4, atol=1e-5)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("checkpoint", [None, "e4m3"])
+def test_routed_layer_with_one_expert(checkpoint, dtype):
+    """Rows of x's type with float32 parameters are taken as with more experts, and the checkpoint is kept."""
+    torch.manual_seed(6)
+    layer = BatchedExpertMoE(2, 8, 2, 1, True, 2, residual_norm=False, routed=True, checkpoint=checkpoint)
+    x = torch.randn(2, 5, 8).to(dtype).requires_grad_(True)
+    y = layer(x)
+    dy = torch.randn(2, 5, 8).to(dtype)
+    dx, dw = torch.autograd.grad(y, (x, layer.w_up), dy)
+    assert y.dtype == dtype and dx.dtype == dtype and dw.dtype == torch.float32
+    ref = {n: p.detach().to(dtype).double() for n, p in layer.named_parameters()}
+    xd = x.detach().double()
+    h = torch.einsum("dbi,dih->dbh", xd, ref["w_up"][:, 0]) + ref["b_up"]
+    z = h[..., :16] * torch.nn.functional.silu(h[..., 16:])
+    want = torch.einsum("dbh,dhi->dbi", z, ref["w_down"][:, 0]) + ref["b_down"]
+    dz = torch.einsum("dbi,dhi->dbh", dy.double(), ref["w_down"][:, 0])
+    at = e4m3_checkpoint_reference(h.to(dtype).reshape(-1, 32)).double().view_as(h) if checkpoint else h
+    s = torch.sigmoid(at[..., 16:])
+    dh = torch.cat([dz * at[..., 16:] * s, dz * at[..., :16] * s * (1 + at[..., 16:] * (1 - s))], -1)
+    # at most six roundings to x's type lie between input and output, as in the test of the block on CUDA
+    tol = 6 * torch.finfo(dtype).eps / 2 + (1e-5 if dtype == torch.float32 else 0)
+    for got, exact in ((y, want), (dx, torch.einsum("dbh,dih->dbi", dh, ref["w_up"][:, 0])), (dw[:, 0], torch.einsum("dbi,dbh->dih", xd, dh))):
+        assert float((got.detach().double() - exact).norm() / exact.norm()) < tol
+    full = BatchedExpertMoE(2, 8, 2, 1, True, 2, routed=True, checkpoint=checkpoint)  # with the norm: x's type as well
+    assert full(x).dtype == dtype
+    assert full(x[:, :0]).shape == (2, 0, 8)
+
+
+def test_one_expert_keeps_the_checkpoint_and_not_the_activation():
+    held = []
+
+    def pack(t):
+        held.append(t)
+        return t
+
+    layer = BatchedExpertMoE(1, 8, 2, 1, True, 2, residual_norm=False, routed=True, checkpoint="e4m3")
+    x = torch.randn(1, 300, 8).bfloat16()
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+        layer(x)
+    up_gate = torch.einsum("dbi,deih->dbeh", x, layer.w_up.bfloat16()) + layer.b_up.bfloat16().unsqueeze(1)
+    kept = e4m3_checkpoint_reference(up_gate.reshape(-1, 32))
+    assert any(t.shape == kept.shape and torch.equal(t, kept) for t in held)  # on the CPU: the values that it stands for
+    assert not any(t.numel() == up_gate.numel() and torch.equal(t.reshape(-1), up_gate.reshape(-1)) for t in held)
+
+
+def test_routed_mixers_at_their_default_number_of_experts():
+    torch.manual_seed(7)
+    for cls in (TokenMixLargeMoe, TokenMixLargePreGateNoPool):
+        mix = cls(1, 4, 24, head_num=6, scale_size=2, sparse=True, routed=True, checkpoint="e4m3")
+        for dtype in (torch.bfloat16, torch.float32):
+            y = mix(torch.randn(3, 4, 24).to(dtype))
+            assert y.dtype == dtype and torch.isfinite(y).all()
+
+
 def test_no_tokens():
     route = route_topk(torch.empty(2, 0, 3), 2)
     assert route.offsets.tolist() == [0] * 7 and route.rows.numel() == 0

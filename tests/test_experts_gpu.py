@@ -651,6 +651,30 @@ def test_routed_mixer_runs_in_half_types(cuda):
         assert torch.isfinite(x.grad).all() and all(torch.isfinite(p.grad).all() for p in mix.parameters())
 
 
+@pytest.mark.parametrize("dtype,width", [(BF16, 64), (FP16, 64), (BF16, 12), (FP32, 12)])
+@pytest.mark.parametrize("checkpoint", [None, "e4m3"])
+def test_routed_layer_with_one_expert(cuda, checkpoint, dtype, width):
+    """Nothing to route: any width and type, and the checkpoint is kept; outputs and gradients against 64 bits."""
+    torch.manual_seed(2)
+    layer = BatchedExpertMoE(2, width, 2, 1, True, 2, residual_norm=False, routed=True, checkpoint=checkpoint).to(cuda)
+    h = 2 * width
+    x, dy = torch.randn(2, 90, width, device=cuda).to(dtype).requires_grad_(True), torch.randn(2, 90, width, device=cuda).to(dtype)
+    y = layer(x)
+    assert y.dtype == dtype
+    dx, dw = torch.autograd.grad(y, (x, layer.w_up), dy)
+    wu, wd = (p.detach().to(dtype).double()[:, 0] for p in (layer.w_up, layer.w_down))
+    u = torch.einsum("dbi,dih->dbh", x.detach().double(), wu)
+    want = torch.einsum("dbh,dhi->dbi", u[..., :h] * torch.nn.functional.silu(u[..., h:]), wd)
+    dz = torch.einsum("dbi,dhi->dbh", dy.double(), wd)
+    at = e4m3_checkpoint_reference(u.to(dtype).reshape(-1, 2 * h).cpu()).to(cuda).double().view_as(u) if checkpoint else u
+    s = torch.sigmoid(at[..., h:])
+    du = torch.cat([dz * at[..., h:] * s, dz * at[..., :h] * s * (1 + at[..., h:] * (1 - s))], -1)
+    # six roundings of half a step, as for the block; float32 sums of a few hundred products beside them
+    tol = 6 * torch.finfo(dtype).eps / 2 + 512 * 2 ** -23
+    for got, exact in ((y, want), (dx, torch.einsum("dbh,dih->dbi", du, wu)), (dw[:, 0], torch.einsum("dbi,dbh->dih", x.detach().double(), du))):
+        assert float((got.detach().double() - exact).norm() / exact.norm()) < tol
+
+
 # ------------------------------------------------------------------ refusals
 def test_no_rows(cuda):
     w = torch.randn(3, 16, 24, device=cuda).to(BF16).requires_grad_(True)
