@@ -666,7 +666,11 @@ def test_routed_layer_with_one_expert(cuda, checkpoint, dtype, width):
     u = torch.einsum("dbi,dih->dbh", x.detach().double(), wu)
     want = torch.einsum("dbh,dhi->dbi", u[..., :h] * torch.nn.functional.silu(u[..., h:]), wd)
     dz = torch.einsum("dbi,dhi->dbh", dy.double(), wd)
-    at = e4m3_checkpoint_reference(u.to(dtype).reshape(-1, 2 * h).cpu()).to(cuda).double().view_as(u) if checkpoint else u
+    if checkpoint:  # of the activation as the layer has it: one that lies on a border of e4m3 rounds to either side
+        own = torch.einsum("dbi,deih->dbeh", x.detach(), layer.w_up.detach().to(dtype)) + layer.b_up.detach().to(dtype).unsqueeze(1)
+        at = e4m3_checkpoint_reference(own.reshape(-1, 2 * h).cpu()).to(cuda).double().view_as(u)
+    else:
+        at = u
     s = torch.sigmoid(at[..., h:])
     du = torch.cat([dz * at[..., h:] * s, dz * at[..., :h] * s * (1 + at[..., h:] * (1 - s))], -1)
     # six roundings of half a step, as for the block; float32 sums of a few hundred products beside them
