@@ -486,7 +486,9 @@ class BatchedExpertMoE(nn.Module):
         self.norm_scale = nn.Parameter(torch.ones(batch_dim, in_dim))
 
     def _forward_routed(self, x: torch.Tensor) -> torch.Tensor:
-        logits = torch.einsum("dbi,dio->dbo", x, self.w_gate.to(x.dtype)) + self.b_gate.to(x.dtype).unsqueeze(1)
+        # the router in the wider of x's and the gate's types: rounded to 16 bits, close logits of a float32 gate would tie
+        wide = torch.promote_types(x.dtype, torch.promote_types(self.w_gate.dtype, self.b_gate.dtype))
+        logits = torch.einsum("dbi,dio->dbo", x.to(wide), self.w_gate.to(wide)) + self.b_gate.to(wide).unsqueeze(1)
         moe = expert_mlp(x, logits, self.w_up, self.b_up, self.w_down, self.b_down, top_k=self.top_k,
                          checkpoint=self.checkpoint)
         if self.residual_norm:

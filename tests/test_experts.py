@@ -184,6 +184,31 @@ def test_token_mixers_pass_the_option_on():
         torch.testing.assert_close(b(x), a(x), rtol=1e-4, atol=1e-5)
 
 
+def test_routed_layer_decides_in_the_type_of_a_float32_gate():
+    """Logits that are equal in 16 bits and not in float32, and gradients of the gate, with 16-bit rows."""
+    layer = BatchedExpertMoE(1, 8, 1, 4, True, 1, residual_norm=False, routed=True)
+    with torch.no_grad():
+        for p in (layer.w_gate, layer.w_down):
+            p.zero_()
+        layer.b_gate.copy_(torch.tensor([[8.0, 8.01, 0.0, 8.005]]))
+        layer.b_down.copy_(torch.arange(4.0).view(1, 4, 1).expand(1, 4, 8))
+        assert torch.equal(layer(torch.randn(1, 3, 8).bfloat16()), torch.ones(1, 3, 8).bfloat16())  # expert 1
+        layer.b_gate.zero_()
+        layer.w_gate[0, :, 2], layer.w_gate[0, :, 0] = 1.0, 1.0 - 2.0 ** -10
+        assert torch.equal(layer(torch.ones(1, 3, 8).bfloat16()), torch.full((1, 3, 8), 2.0).bfloat16())
+    torch.manual_seed(8)
+    layer = BatchedExpertMoE(2, 8, 2, 5, True, 2, residual_norm=False, routed=True)
+    exact = BatchedExpertMoE(2, 8, 2, 5, True, 2, residual_norm=False, routed=True).double()
+    exact.load_state_dict(layer.state_dict())
+    x, dy = torch.randn(2, 40, 8).bfloat16(), torch.randn(2, 40, 8).bfloat16()
+    layer(x).backward(dy)
+    exact(x.double()).backward(dy.double())
+    # the experts' rows come in bfloat16: six roundings of half a step in the norm, as for the block
+    for n in ("w_gate", "b_gate"):
+        got, want = getattr(layer, n).grad.double(), getattr(exact, n).grad
+        assert float((got - want).norm() / want.norm()) < 6 * 2 ** -8, n
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("checkpoint", [None, "e4m3"])
 def test_routed_layer_with_one_expert(checkpoint, dtype):
