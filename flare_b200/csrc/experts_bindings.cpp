@@ -573,7 +573,7 @@ Tensor combine_rows_op(const Tensor& z, const optional<Tensor>& weights, const T
   const Tensor v = unit_rows(z);
   optional<Tensor> w;
   if (weights.has_value()) {
-    value_check(weights->numel() == row_of.numel(), "weights must have the shape ", row_of.sizes(), ", got ", weights->sizes());
+    value_check(weights->numel() == row_of.numel() && weights->dim() >= 1 && weights->size(-1) == row_of.size(-1), "weights must have the shape ", row_of.sizes(), ", got ", weights->sizes());
     same_device(z, *weights);
     w = weights->to(at::kFloat).contiguous();
   }

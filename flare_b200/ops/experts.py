@@ -249,7 +249,7 @@ def combine_rows_reference(z, route: ExpertRoute, weights=None):
 def combine_rows(z: torch.Tensor, route: ExpertRoute, weights: torch.Tensor | None = None) -> torch.Tensor:
     """``y[t] = sum_j weights[t, j] * z[row_of[t, j]]``: rows ``[R, n]`` of a route back to its tokens ``[tokens, n]``.
 
-    ``weights`` (``route.weights``, or any of its shape) may be left out for the plain sum.  Sums are in float32, in
+    ``weights`` (``route.weights``, or any ``[.., tokens, k]``) may be left out for the plain sum.  Sums are in float32, in
     order of ``j``; a token without rows gets zeros.
     """
     if z.is_cuda:
@@ -258,7 +258,7 @@ def combine_rows(z: torch.Tensor, route: ExpertRoute, weights: torch.Tensor | No
         raise ValueError(f"z must be [{route.row_of.numel()}, n] for this route, got {tuple(z.shape)}")
     if route.offsets.dtype != torch.int32 or route.offsets.dim() != 1 or not route.offsets.numel():
         raise ValueError(f"offsets must be int32 [groups + 1], got {route.offsets.dtype} {tuple(route.offsets.shape)}")
-    if weights is not None and weights.numel() != route.row_of.numel():
+    if weights is not None and (weights.numel() != route.row_of.numel() or weights.shape[-1:] != route.row_of.shape[-1:]):
         raise ValueError(f"weights must have the shape {tuple(route.row_of.shape)}, got {tuple(weights.shape)}")
     on_cuda(z, route.row_of, *(() if weights is None else (weights,)))  # refuses a mixture of devices
     return combine_rows_reference(z, route, weights)

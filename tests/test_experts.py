@@ -388,6 +388,21 @@ def test_native_refusals_of_tangents():
                     call(lambda v: v.clone().requires_grad_(leaf))
 
 
+def test_combination_refuses_weights_of_another_layout():
+    """As many values in another layout (choices first) are not the weights of these choices."""
+    from flare_b200._native import available, native
+
+    route = route_topk(torch.randn(2, 3, 4), 2)
+    z, w = torch.randn(12, 5), route.weights
+    assert torch.equal(combine_rows(z, route, w.reshape(6, 2)), combine_rows(z, route, w))
+    for bad in (w.reshape(6, 2).t(), w.reshape(-1), w.reshape(2, 2, 3)):
+        with pytest.raises(ValueError, match="weights must have the shape"):
+            combine_rows(z, route, bad)
+        if available():
+            with pytest.raises(ValueError, match="weights must have the shape"):
+                native().combine_rows(z, bad, route.offsets, route.row_of)
+
+
 def test_first_call_in_a_capture_is_refused(monkeypatch):
     from flare_b200 import _native
     from flare_b200.ops import experts
