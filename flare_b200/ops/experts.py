@@ -242,7 +242,8 @@ def combine_rows_reference(z, route: ExpertRoute, weights=None):
     zf = torch.cat([z.to(acc), z.new_zeros(1, z.shape[1], dtype=acc)])
     picked = torch.where(on, zf[torch.where(at >= 0, at, z.shape[0])], torch.zeros((), dtype=acc, device=z.device))
     if weights is not None:
-        picked = picked * weights.reshape(-1, k, 1).to(acc)
+        w = weights.reshape(-1, k, 1).to(acc)
+        picked = picked * torch.where(on, w, torch.zeros_like(w))  # what stands where there is no choice is not used
     return picked.sum(1).to(z.dtype)
 
 

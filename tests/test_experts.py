@@ -403,6 +403,17 @@ def test_combination_refuses_weights_of_another_layout():
                 native().combine_rows(z, bad, route.offsets, route.row_of)
 
 
+def test_combination_ignores_weights_where_there_is_no_choice():
+    route = route_topk(torch.tensor([[0.0, 1.0, -math.inf], [-math.inf] * 3, [-math.inf, 2.0, -math.inf]]), 2)
+    z = torch.ones(6, 4, requires_grad=True)
+    for bad in (math.nan, math.inf):
+        w = torch.where(route.experts < 0, bad, route.weights).requires_grad_(True)
+        y = combine_rows(z, route, w)
+        assert torch.equal(y, combine_rows(z, route, route.weights))
+        dz, dw = torch.autograd.grad(y, (z, w), torch.ones_like(y))
+        assert torch.isfinite(dz).all() and torch.isfinite(dw).all() and not dw[route.experts < 0].any()
+
+
 def test_first_call_in_a_capture_is_refused(monkeypatch):
     from flare_b200 import _native
     from flare_b200.ops import experts

@@ -497,6 +497,17 @@ def test_combine_views(cuda):
         assert torch.equal(combine_rows(z, route, w), combine_rows(z.contiguous(), route, w.float()))
 
 
+def test_combination_ignores_weights_where_there_is_no_choice(cuda):
+    route = route_topk(torch.tensor([[0.0, 1.0, -math.inf], [-math.inf] * 3, [-math.inf, 2.0, -math.inf]], device=cuda), 2)
+    z = torch.ones(6, 4, device=cuda, requires_grad=True)
+    for bad in (math.nan, math.inf):
+        w = torch.where(route.experts < 0, bad, route.weights).requires_grad_(True)
+        y = combine_rows(z, route, w)
+        assert torch.equal(y, combine_rows(z, route, route.weights))
+        dz, dw = torch.autograd.grad(y, (z, w), torch.ones_like(y))
+        assert torch.isfinite(dz).all() and torch.isfinite(dw).all() and not dw[route.experts < 0].any()
+
+
 # ------------------------------------------------------------ used together
 def plain_mlp(x, lg, wu, bu, wd, bd, k, checkpoint):
     """The block in 64 bits from the definition, its activations rounded where the kernels store them (rounding passes
