@@ -312,6 +312,28 @@ def test_grouped_linear_in_slices(cuda, R, G):
     within(p._flare_grad, 1 + dw0, (R + 3) * 2 ** -23 * (1 + aw), "accumulated")
 
 
+@pytest.mark.parametrize("N", [8, 72, 520])
+@pytest.mark.parametrize("sizes", [
+    [9000], [8193], [31, 1, 32, 33, 63, 64, 65, 0, 127, 129, 95, 10000], [8191, 1, 0, 8192, 64, 1, 63], [5000, 5000],
+    [160 * 7 + 1, 160 * 9 - 1, 160, 20000, 159, 161, 0], [(i * 13) % 67 for i in range(520)], [1] * 17 + [4095, 4097, 513, 511]])
+def test_grouped_linear_sums_lose_no_row(cuda, sizes, N):
+    """Weight and bias gradients of small whole numbers are exact in float32 whatever the order: groups that end just before,
+    on and after the borders of steps, chunks and slices, written in float32 and added to a flat buffer."""
+    gen = torch.Generator(device="cuda").manual_seed(N + len(sizes))
+    off = offsets_of(sizes, 2, cuda)
+    R, G, K = 2 + sum(sizes) + 3, len(sizes), 40
+    x, dy = (torch.randint(-3, 4, (R, n), device=cuda, generator=gen).to(BF16) for n in (K, N))
+    w, b = (torch.randn(G, *n, device=cuda, generator=gen).requires_grad_(True) for n in ((K, N), (N,)))
+    dw, db = torch.autograd.grad(grouped_linear(x, w, b, offsets=off), (w, b), dy)
+    assert dw.dtype == db.dtype == FP32
+    _, _, (dw0, _), (db0, _) = exact_linear(x, w.detach(), b.detach(), off, dy)  # sums below 2^18
+    assert torch.equal(dw.double(), dw0) and torch.equal(db.double(), db0)
+    p, q = torch.nn.Parameter(w.detach()), torch.nn.Parameter(b.detach())
+    p._flare_grad, q._flare_grad = torch.full_like(p, 5.0), torch.full_like(q, -7.0)
+    grouped_linear(x, p, q, offsets=off).backward(dy)
+    assert torch.equal(p._flare_grad.double(), dw0 + 5) and torch.equal(q._flare_grad.double(), db0 - 7)
+
+
 def test_grouped_linear_frozen_operands(cuda):
     """Only what requires a gradient gets one: the bias alone, the input alone, the weight alone."""
     route = route_topk(torch.randn(300, 4, device=cuda), 2)
