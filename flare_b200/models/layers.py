@@ -464,6 +464,8 @@ class BatchedExpertMoE(nn.Module):
     ones, in x's type (float32 too) and of any width, and the checkpoint is kept as asked.
     """
 
+    routed, checkpoint = False, None  # of layers pickled whole before they had these
+
     def __init__(self, batch_dim: int, in_dim: int, scale_size: int, num_experts: int, sparse: bool, top_k: int,
                  residual_norm: bool = True, routed: bool = False, checkpoint: str | None = None):
         super().__init__()

@@ -264,6 +264,21 @@ def test_routed_mixers_at_their_default_number_of_experts():
             assert y.dtype == dtype and torch.isfinite(y).all()
 
 
+def test_layers_pickled_without_the_options_still_run():
+    import io
+
+    torch.manual_seed(9)
+    layer = BatchedExpertMoE(2, 8, 2, 3, True, 2)
+    x = torch.randn(2, 5, 8)
+    want = layer(x)
+    for name in ("routed", "checkpoint"):
+        layer.__dict__.pop(name, None)
+    held = io.BytesIO()
+    torch.save(layer, held)
+    held.seek(0)
+    assert torch.equal(torch.load(held, weights_only=False)(x), want)
+
+
 def test_no_tokens():
     route = route_topk(torch.empty(2, 0, 3), 2)
     assert route.offsets.tolist() == [0] * 7 and route.rows.numel() == 0
