@@ -630,6 +630,9 @@ void launch(const GroupedArgs& a, cudaStream_t s, int slices = 1) {
 // The weight gradient's tiles are as wide as N allows.  A few groups of a small weight and many
 // rows leave most of the machine idle: their rows are cut into slices of at least 512 rows of an
 // average group, about two tiles for each SM (33 us against 630 us for 131072 x 64 x 128 in 2 groups).
+// And whatever the groups, a slice has 2^25 rows at most: one group may have nearly all of them, and
+// the waits for a tile's end are bounded by time.
+constexpr int64_t kMaxSliceRows = 1 << 25;
 struct WgradShape {
   int bn, slices;
 };
@@ -637,7 +640,7 @@ WgradShape wgrad_shape(int G, int64_t R, int K, int N) {
   WgradShape w;
   w.bn = N > 128 ? 256 : N > 64 ? 128 : 64;
   const int64_t tiles = static_cast<int64_t>(G) * ceil_div(K, 128) * ceil_div(N, w.bn);
-  w.slices = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(64, R / G / 512), 296 / tiles)));
+  w.slices = static_cast<int>(std::max<int64_t>({1, ceil_div(R, kMaxSliceRows), std::min<int64_t>({64, R / G / 512, 296 / tiles})}));
   return w;
 }
 

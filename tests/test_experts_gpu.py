@@ -334,6 +334,26 @@ def test_grouped_linear_sums_lose_no_row(cuda, sizes, N):
     assert torch.equal(p._flare_grad.double(), dw0 + 5) and torch.equal(q._flare_grad.double(), db0 - 7)
 
 
+def test_grouped_linear_very_long_group(cuda):
+    """One of 300 groups has nearly all of 70 million rows: cut into slices (its sums of small whole numbers are exact)."""
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    sizes = [i % 3 for i in range(150)] + [70_000_000] + [i % 5 for i in range(149)]
+    off = offsets_of(sizes, 0, cuda)
+    R = sum(sizes)
+    x, dy = (torch.randint(-3, 4, (R, 8), device=cuda, generator=gen, dtype=torch.int8).to(BF16) for _ in range(2))
+    w, b = torch.zeros(300, 8, 8, device=cuda, requires_grad=True), torch.zeros(300, 8, device=cuda, requires_grad=True)
+    dw, db = torch.autograd.grad(grouped_linear(x, w, b, offsets=off), (w, b), dy)
+    default_status(cuda).check()
+    at = off.tolist()
+    for g in (149, 150, 151, 299):
+        want, sums = torch.zeros(8, 8, dtype=torch.float64, device=cuda), torch.zeros(8, dtype=torch.float64, device=cuda)
+        for lo in range(at[g], at[g + 1], 1 << 22):
+            hi = min(lo + (1 << 22), at[g + 1])
+            want += x[lo:hi].double().t() @ dy[lo:hi].double()
+            sums += dy[lo:hi].double().sum(0)
+        assert torch.equal(dw[g].double(), want) and torch.equal(db[g].double(), sums)
+
+
 def test_grouped_linear_frozen_operands(cuda):
     """Only what requires a gradient gets one: the bias alone, the input alone, the weight alone."""
     route = route_topk(torch.randn(300, 4, device=cuda), 2)
