@@ -166,9 +166,11 @@ __device__ __forceinline__ int warp_exclusive(int* tot, int E) {
 }
 
 // Many tokens take three passes (131071 tokens of 128 fp32 logits, four choices: 41 + 5 + 8 us for 67
-// MB read, 10 us at the measured copy: the picks are bound by their instructions, four tokens to a
-// warp; the gradient 13 us for 67 MB written).  With the prefix over all blocks' counts in every
-// block of a second pass instead of a pass of its own, the placing alone took 42 us.
+// MB read, 10 us at the measured copy; the gradient 13 us for 67 MB written).  The picks, four tokens
+// to a warp, are bound by their instructions where they run (ncu: stalls are "not selected" and the
+// math pipe, memory waits a tenth of these; 60 % of issue slots, since 512 blocks are three or four
+// to an SM).  With the prefix over all blocks' counts in every block of a second pass instead of a
+// pass of its own, the placing alone took 42 us.
 // Pass 1: experts and weights of every token of a sub-block (block = slot * chunks + chunk), and
 // its counts: work[slot][chunk][E].
 template <typename T, int LANES, int NV>
@@ -474,9 +476,12 @@ __device__ __forceinline__ void unpack_e4m3(const uint8_t* in, float scale, floa
   }
 }
 
-// Bound by memory and, nearly as much, by the instructions of the sigmoid and the rounding (ncu:
-// 72 % of issue slots): conversions go in pairs.  131072 rows of 2 x 2048 bf16 with the checkpoint:
-// forward 390 us, backward 387 us, 2.16 GB each (5.6 TB/s, 0.85 of the measured copy).
+// Bound by memory and, nearly as much, by the instructions of the sigmoid and the rounding, although
+// conversions go in pairs (ncu, 32768 rows: 77 and 73 % of issue slots, DRAM at 65 %, stalls waiting
+// for memory first).  131072 rows of 2 x 2048 bf16 with the checkpoint: forward 358 to 380 us, backward
+// 370 to 390 us, 2.16 GB each (5.5 to 6.0 TB/s, 0.85 to 0.92 of the measured copy); without it 243
+// (1.61 GB) and 433 us (2.68 GB).  Rows that do not start on 16 bytes go element by element: 131072
+// rows of 2 x 2047 take 1129 and 972 us with the checkpoint, 631 and 955 us without.
 // A thread owns N consecutive columns of up and the same of gate; kGroupCols / N lanes share a
 // scale.  A row's columns are padded to whole scale groups (`cols` chunks of N), short rows share
 // a block.  One pass: x is read once, y and the checkpoint are written once.
@@ -640,8 +645,9 @@ void swiglu_dispatch(const SwigluParams& p, bool backward, cudaStream_t s) {
 }
 
 // ------------------------------------------------------------- combination
-// Bound by memory: 65536 tokens of 512 bf16, two rows each: forward 48 us for 201 MB (0.64 of the
-// measured copy; short rows, random order), backward 54 us for 336 MB (0.95).
+// Bound by memory: 65536 tokens of 512 bf16, two rows each: forward 50 us for 201 MB (0.62 of the
+// measured copy; rows of 1 KB in the order of the groups), backward 56 us for 336 MB (0.92).  Rows
+// that do not start on 16 bytes go element by element: 511 columns take 123 and 145 us.
 // A thread owns N columns of two tokens at a time (of one where z is fp32: its registers are full)
 // and reads their rows, KU of each in flight.
 template <typename T, int N, typename O, int KU>

@@ -64,7 +64,7 @@ struct CombineParams {
   void* y;          // [T, N] contiguous
   const void* dy;   // backward: [T, N], row pitch lddy
   int64_t lddy;
-  void* dz;         // backward: [R, N] contiguous, or null
+  void* dz;         // backward: [R, N] contiguous
   float* dw;        // backward: [T, k]
   const int* total;  // rows in use (the last offset)
 };

@@ -615,6 +615,8 @@ Tensor grouped_linear_op(const Tensor& x, const Tensor& weight, const optional<T
   const Tensor v = tma_rows(x);
   optional<Tensor> b;
   if (bias.has_value()) b = bias->contiguous();
+  // A float32 weight is rounded in every call, whichever groups have rows: nothing is kept from one call
+  // to the next, since the parameter may have changed in between.
   Tensor w = weight.detach().reshape({groups, K, N}).to(x.scalar_type()).contiguous();
   if (reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 != 0) w = w.clone();
   if (wants({&v, &weight}) || (b.has_value() && wants({&*b})))

@@ -27,12 +27,14 @@
 // groups, 177 us against 155 us for 200000 x 256 x 1024 in 64).  A tile that reaches
 // past its group loads only the sixteens of rows that the group has.
 //
-// Measured on one B200, 131072 rows, 512 -> 4096, 32 groups of unequal size, bf16 (550
-// GFLOP a direction): forward 492 us, input gradient 465 us, weight gradient 493 us
-// (1.12 to 1.18 PFLOP/s; cuBLAS on one product of the same size, without groups: 448, 368
-// and 404 us).  The power limit bounds both: 965 to 1000 W, SM clocks at 1.3 to 1.5 GHz
-// of 1.97.  96 groups of 341 rows on average, 2048 -> 512, fp16: 90, 82 and 100 us for
-// 369 MB each, 57 us at the measured copy bandwidth.
+// Measured on B200s, 131072 rows, 512 -> 4096, 32 groups of unequal size, bf16 (550 GFLOP
+// a direction), in a training pass: forward 480 to 500 us, input gradient 455 to 472 us,
+// weight gradient 485 to 511 us (1.08 to 1.21 PFLOP/s, 0.66 to 0.74 of the measured burst);
+// each back to back for seconds 605, 516 and 601 us (0.66, 0.78 and 0.67 of the measured
+// sustained rate).  cuBLAS on one product of the same size, without groups: 448, 368 and 404
+// us, back to back 580, 461 and 509 us.  The power limit bounds both: 965 to 1000 W, SM
+// clocks at 1.3 to 1.5 GHz of 1.97.  96 groups of 341 rows on average, 2048 -> 512, fp16:
+// 90, 82 and 103 us for 369 MB each, 57 us at the measured copy bandwidth.
 // Every sum is held in fp32 and rounded once.  Every wait is bounded.
 #include "experts.cuh"
 #include "gemm.cuh"
@@ -722,8 +724,9 @@ __device__ __forceinline__ void store_any(void* p, int64_t i, int dtype, float v
 // (a cluster's CTAs share the columns and K).  A thread owns 8 columns (one 16-byte load of a
 // weight row) of every 32nd row of the slice and up to MR rows of x; its partial sums meet by
 // shuffles, then through shared memory, then across the cluster, always in the same order.
-// Eight rows in as many groups of 16, 512 -> 4096: 8.1 us for 34 MB of weights (5.2 us at the
-// measured copy bandwidth; the launch is about 2); 2048 -> 512: 8.8 us for 17 MB.
+// Eight rows in as many groups of 16, 512 -> 4096: 7.2 us for 34 MB of weights (5.2 us at the
+// measured copy bandwidth; the launch is about 2); 2048 -> 512: 7.1 us for 17 MB.  Both with the
+// weights in L2, one launch after another.
 constexpr int kFewK = 512;  // a chunk of K whose x values are in shared memory
 constexpr int kFewRows = 4; // of a group at a time: 32 sums a thread, three blocks on an SM
 template <typename T, int MR>
@@ -898,8 +901,8 @@ void few_rows_launch(const GroupedArgs& a, cudaStream_t s) {
 // segment of its own, number chunk + group: one of the two grows from a segment to the next.  A
 // second kernel adds a group's segments in order.
 // Up to kSumOneLaunch rows: one kernel, block = 64 columns of a slice of one group, slices of a
-// group a cluster, added in order (3003 x 328: 4.8 us against 12 us for the two).
-// 131072 x 4096: 180 us, 1.07 GB at 6.0 TB/s.  Added up by warps of the weight gradient from its
+// group a cluster, added in order (3003 x 328: 4.8 us against 12 us for the two kernels).
+// 131072 x 4096: 173 + 9 us, 1.07 GB at 5.9 TB/s.  Added up by warps of the weight gradient from its
 // stages instead, the columns cost that kernel 120 to 150 us: its four stages could not spare them.
 constexpr int64_t kSumOneLaunch = 8192;
 int sum_rows(int64_t R, int cols) {  // about eight blocks for each SM

@@ -54,7 +54,8 @@ def _status(x: torch.Tensor) -> int:
 
 
 class ExpertRoute(NamedTuple):
-    """Where tokens go.  ``k`` choices a token, ``R = tokens * k`` row places in all."""
+    """Where tokens go.  ``k`` choices a token, ``R = tokens * k`` row places in all.  The five belong together: the
+    operators check their types and sizes, not that ``rows``, ``row_of`` and ``offsets`` say the same."""
 
     experts: torch.Tensor  # int32 [.., tokens, k]: the chosen experts by falling logit, -1 where there is none
     weights: torch.Tensor  # float32 [.., tokens, k]: softmax over the chosen logits, 0 where there is none
@@ -271,7 +272,9 @@ def expert_mlp(x: torch.Tensor, logits: torch.Tensor, w_up: torch.Tensor, b_up: 
     """A routed mixture of SwiGLU experts: ``y[t] = sum_j w_tj (swiglu(x[t] W_up[e_tj] + b_up) W_down[e_tj] + b_down)``.
 
     ``x [.., d]`` and ``logits [.., experts]`` have the same leading shape (``[tokens]`` or ``[slots, tokens]``); weights
-    ``[.., d, 2h]`` and ``[.., h, d]``, biases ``[.., 2h]`` and ``[.., d]``, a matrix for each expert of each slot.
+    ``[.., d, 2h]`` and ``[.., h, d]``, biases ``[.., 2h]`` and ``[.., d]``, a matrix for each expert of each slot.  On CUDA
+    the limits are those of ``grouped_linear``: 16-bit x, widths in multiples of 8, at most ``MAX_GROUPS`` experts over all
+    slots.  Float32 weights are rounded in every call; where that counts (a serving step of a few tokens), pass 16-bit ones.
     """
     if x.shape[:-1] != logits.shape[:-1]:
         raise ValueError(f"x and logits must have the same tokens, got {tuple(x.shape)} and {tuple(logits.shape)}")
